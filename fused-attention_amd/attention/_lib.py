@@ -29,6 +29,9 @@ FA_ERR_LAUNCH = -6
 FA_ERR_UNSUPPORTED = -7
 FA_ERR_WORKSPACE = -8
 FA_ERR_SCRATCH = -9
+FA_ERR_LAYOUT = -10
+FA_ERR_ROTATION = -11
+FA_ERR_PAGES = -12
 
 # (name, restype, argtypes) for every symbol of include/fa.h
 _VP, _I, _F = ctypes.c_void_p, ctypes.c_int, ctypes.c_float
@@ -40,6 +43,13 @@ SIGNATURES = {
                         _I, _I, _I, _I, _I, _I, _F, _F, _I, _I, _VP, ctypes.c_size_t, _VP]),
     "fa_bwd_gqa_noalloc": (_I, [_VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP,
                                 _I, _I, _I, _I, _I, _I, _F, _F, _I, _I, _VP]),
+    "fa_qk_norm_rotary": (_I, [_VP, _VP, _VP, _VP, _VP, _I, _I, _I, _I, _I, _I, _VP]),
+    "fa_qk_norm_rotary_bwd": (_I, [_VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP,
+                                   _I, _I, _I, _I, _I, _I, _VP, ctypes.c_size_t, _VP]),
+    "fa_qk_norm_rotary_workspace_size": (ctypes.c_size_t, [_I, _I, _I, _I, _I]),
+    "fa_paged_append": (_I, [_VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _I, _I, _I, _I, _I, _VP]),
+    "fa_paged_attention": (_I, [_VP, _VP, _VP, _VP, _VP, _VP, _I, _I, _I, _I, _I, _F, _VP, ctypes.c_size_t, _VP]),
+    "fa_paged_attention_workspace_size": (ctypes.c_size_t, [_I, _I, _I, _I, _I, ctypes.c_longlong]),
     "fa_noalloc_scratch_bytes": (ctypes.c_size_t, []),
     "fa_fwd_exact": (_I, [_VP, _VP, _VP, _VP, _VP, _I, _I, _I, _I, _I, _I, _F, _I, _I, _I, _VP]),
     "fa_bwd_gqa_exact": (_I, [_VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP,
@@ -155,7 +165,7 @@ def check(code, what):
     if code == FA_ERR_DTYPE:
         raise TypeError(msg)
     if code in (FA_ERR_DIMS, FA_ERR_HEADDIM, FA_ERR_TILE, FA_ERR_NULL, FA_ERR_UNSUPPORTED, FA_ERR_WORKSPACE,
-                FA_ERR_SCRATCH):
+                FA_ERR_SCRATCH, FA_ERR_LAYOUT, FA_ERR_ROTATION, FA_ERR_PAGES):
         raise ValueError(msg)
     raise RuntimeError(msg)
 

@@ -76,6 +76,40 @@ int check_common(int B, int H, int S, int D, int dtype, int block_m, int block_n
   return FA_OK;
 }
 
+// What the calls on strided rows share (norm and rotation, paged cache).
+int check_rows_call(int B, int H, int H_kv, int N, int D, int dtype) {
+  if (H_kv <= 0 || (long long)B * H_kv * N > 0x7fffffffLL) return FA_ERR_DIMS;
+  return check_common(B, H, N, D, dtype, 64, 64);
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+int check_rows(const fa_rows& r) {
+  if (!r.data) return FA_ERR_NULL;
+  return aligned16(r.data) && ((r.stride_b | r.stride_h | r.stride_n) & 7) == 0 ? FA_OK : FA_ERR_LAYOUT;
+}
+
+int check_rotation(const fa_rotation& r, int D, int dtype) {
+  if ((r.q_weight || r.k_weight) && r.weight_dtype != dtype && r.weight_dtype != FA_F32) return FA_ERR_ROTATION;
+  if (!r.table) return FA_OK;
+  if (!aligned16(r.table) || r.table_len <= 0) return FA_ERR_ROTATION;
+  if (r.rotary_dim <= 0 || r.rotary_dim > D || r.rotary_dim % 16 != 0) return FA_ERR_ROTATION;
+  if (r.axes < 1 || r.axes > fa::kMaxAxes || (r.axes > 1 && !r.positions)) return FA_ERR_ROTATION;
+  int last = 0;
+  for (int i = 0; i < r.axes - 1; ++i) {
+    if (r.section_end[i] < last || r.section_end[i] > r.rotary_dim / 2) return FA_ERR_ROTATION;
+    last = r.section_end[i];
+  }
+  return FA_OK;
+}
+
+int check_cache(const fa_paged_cache& c) {
+  if (!c.k || !c.v || !c.k_scale || !c.v_scale || !c.block_table) return FA_ERR_NULL;
+  if (c.page_size != 16 && c.page_size != 32 && c.page_size != 64 && c.page_size != 128) return FA_ERR_PAGES;
+  if (c.num_pages <= 0 || c.table_width <= 0 || c.table_stride < 0 || c.H_kv <= 0) return FA_ERR_PAGES;
+  return aligned16(c.k) && aligned16(c.v) ? FA_OK : FA_ERR_PAGES;
+}
+
 using fa::cu_count;
 using fa::kMaxDevices;
 
@@ -498,6 +532,94 @@ int fa_bwd_gqa_exact(const void* q, const void* k, const void* v, const void* o,
   return fn(a);
 }
 
+int fa_qk_norm_rotary(const fa_rows* q, const fa_rows* k, const fa_rows* q_out, const fa_rows* k_out,
+                      const fa_rotation* rotation, int B, int H, int H_kv, int N, int D, int dtype,
+                      void* hip_stream) {
+  if (!q || !k || !q_out || !k_out || !rotation) return FA_ERR_NULL;
+  int st = check_rows_call(B, H, H_kv, N, D, dtype);
+  if (st == FA_OK) st = check_rotation(*rotation, D, dtype);
+  if (st != FA_OK) return st;
+  if (!rotation->q_weight != !rotation->k_weight) return FA_ERR_ROTATION;
+  for (const fa_rows* r : {q, k, q_out, k_out})
+    if ((st = check_rows(*r)) != FA_OK) return st;
+  fa::QkArgs a{};
+  a.q = *q, a.k = *k, a.oq = *q_out, a.ok = *k_out, a.rot = *rotation;
+  a.B = B, a.H = H, a.Hkv = H_kv, a.N = N, a.stream = hip_stream;
+  return fa::qk_norm_rotary(dtype, D, a);
+}
+
+int fa_qk_norm_rotary_bwd(const fa_rows* q, const fa_rows* k, const fa_rows* gq, const fa_rows* gk,
+                          const fa_rows* dq, const fa_rows* dk, void* dwq, void* dwk,
+                          const fa_rotation* rotation, int B, int H, int H_kv, int N, int D, int dtype,
+                          void* workspace, size_t workspace_bytes, void* hip_stream) {
+  if (!q || !k || !gq || !gk || !dq || !dk || !rotation) return FA_ERR_NULL;
+  int st = check_rows_call(B, H, H_kv, N, D, dtype);
+  if (st == FA_OK) st = check_rotation(*rotation, D, dtype);
+  if (st != FA_OK) return st;
+  if (!rotation->q_weight != !rotation->k_weight) return FA_ERR_ROTATION;
+  for (const fa_rows* r : {q, k, gq, gk, dq, dk})
+    if ((st = check_rows(*r)) != FA_OK) return st;
+  if (rotation->q_weight) {
+    if (!dwq || !dwk || !workspace) return FA_ERR_NULL;
+    if ((reinterpret_cast<uintptr_t>(workspace) & 15) ||
+        workspace_bytes < fa::qk_norm_rotary_workspace(B, H, H_kv, N, D))
+      return FA_ERR_WORKSPACE;
+  }
+  fa::QkArgs a{};
+  a.q = *q, a.k = *k, a.gq = *gq, a.gk = *gk, a.oq = *dq, a.ok = *dk, a.rot = *rotation;
+  a.B = B, a.H = H, a.Hkv = H_kv, a.N = N, a.stream = hip_stream;
+  a.part = static_cast<float*>(workspace), a.dwq = dwq, a.dwk = dwk;
+  return fa::qk_norm_rotary_bwd(dtype, D, a);
+}
+
+size_t fa_qk_norm_rotary_workspace_size(int B, int H, int H_kv, int N, int D) {
+  if (check_rows_call(B, H, H_kv, N, D, FA_F16) != FA_OK) return 0;
+  return fa::qk_norm_rotary_workspace(B, H, H_kv, N, D);
+}
+
+int fa_paged_append(const fa_rows* q, const fa_rows* k, const fa_rows* v, const fa_rows* q_out,
+                    const fa_paged_cache* cache, const int* past_lens, const int* new_lens,
+                    const fa_rotation* rotation, int B, int H, int N, int D, int dtype, void* hip_stream) {
+  if (!k || !v || !cache || !past_lens || !rotation) return FA_ERR_NULL;
+  int st = check_cache(*cache);
+  if (st == FA_OK) st = check_rows_call(B, q ? H : cache->H_kv, cache->H_kv, N, D, dtype);
+  if (st == FA_OK) st = check_rotation(*rotation, D, dtype);
+  if (st == FA_OK) st = check_rows(*k);
+  if (st == FA_OK) st = check_rows(*v);
+  if (st != FA_OK) return st;
+  fa::AppendArgs a{};
+  if (q) {
+    if (!q_out) return FA_ERR_NULL;
+    if ((st = check_rows(*q)) != FA_OK || (st = check_rows(*q_out)) != FA_OK) return st;
+    a.q = *q, a.oq = *q_out;
+  }
+  a.k = *k, a.v = *v, a.rot = *rotation, a.cache = *cache, a.past = past_lens, a.fresh = new_lens;
+  a.B = B, a.H = H, a.N = N, a.D = D, a.stream = hip_stream;
+  return fa::paged_append(dtype, a);
+}
+
+int fa_paged_attention(const fa_rows* q, const fa_paged_cache* cache, const int* past_lens,
+                       const int* new_lens, const fa_rows* o, float* lse, int B, int H, int N, int D,
+                       int dtype, float scale_log2, void* workspace, size_t workspace_bytes, void* hip_stream) {
+  if (!q || !o || !cache || !past_lens) return FA_ERR_NULL;
+  int st = check_cache(*cache);
+  if (st == FA_OK) st = check_rows_call(B, H, cache->H_kv, N, D, dtype);
+  if (st != FA_OK) return st;
+  if (H % cache->H_kv != 0) return FA_ERR_DIMS;
+  if ((st = check_rows(*q)) != FA_OK || (st = check_rows(*o)) != FA_OK) return st;
+  if (reinterpret_cast<uintptr_t>(workspace) & 15) return FA_ERR_WORKSPACE;
+  fa::PagedArgs a{};
+  a.q = *q, a.o = *o, a.cache = *cache, a.past = past_lens, a.fresh = new_lens, a.lse = lse;
+  a.part = static_cast<float*>(workspace);
+  a.B = B, a.H = H, a.N = N, a.D = D, a.scale_log2 = scale_log2, a.stream = hip_stream;
+  return fa::paged_attention(dtype, a, workspace ? workspace_bytes : 0);
+}
+
+size_t fa_paged_attention_workspace_size(int B, int H, int H_kv, int N, int D, long long keys) {
+  if (check_rows_call(B, H, H_kv, N, D, FA_F16) != FA_OK || H % H_kv != 0 || keys <= 0) return 0;
+  return fa::paged_attention_workspace(B, H, H_kv, N, D, keys);
+}
+
 int fa_fwd_heads_per_wg(int B, int H, int H_kv, int S, int D, int block_m, int block_n) {
   if (B <= 0 || H <= 0 || S <= 0 || H_kv <= 0 || H_kv > H || H % H_kv != 0) return 0;
   if (D != 32 && D != 64 && D != 128) return 0;
@@ -544,10 +666,17 @@ const char* fa_strerror(int status) {
     case FA_ERR_SCRATCH:
       return "this shape's per-row terms (8 * B * H * S bytes) exceed the library's device scratch "
              "(fa_bwd_gqa_noalloc); use fa_bwd_gqa with a caller workspace";
+    case FA_ERR_LAYOUT: return "rows must be 16-byte aligned with strides that are multiples of 8";
+    case FA_ERR_ROTATION:
+      return "rotation outside what is supported (rotary_dim a multiple of 16 up to D, 1 to 3 axes with ascending "
+             "sections, aligned fp32 table, weights of the rows' type or fp32)";
+    case FA_ERR_PAGES:
+      return "page cache outside what is supported (page size 16, 32, 64 or 128, at least one page and one "
+             "table column, 16-byte aligned pages)";
     default: return "unknown status";
   }
 }
 
-int fa_version(void) { return 140; }
+int fa_version(void) { return 150; }
 
 }  // extern "C"

@@ -24,6 +24,7 @@
 #include <cmath>
 
 #include "fa.h"
+#include "fa_ops.h"
 
 namespace {
 
@@ -108,4 +109,5 @@ PYBIND11_MODULE(fa_autograd, m) {
   m.def("fused_attention", &fused_attention, "O = attention(q, k, v) with a backward; k, v may have fewer heads",
         pybind11::arg("q"), pybind11::arg("k"), pybind11::arg("v"), pybind11::arg("tile_m"), pybind11::arg("tile_n"));
   m.def("forward", &forward, "fa_fwd of checked tensors on the current stream; returns its status");
+  fa_def_ops(m);
 }

@@ -50,11 +50,62 @@ struct BwdArgs {
   bool small;
 };
 
+// rows [B, heads, N, D] with strides, and their norm and rotation, as the C ABI takes them
+typedef ::fa_rows Rows;
+typedef ::fa_rotation RotaryArgs;
+constexpr int kMaxAxes = 3;
+
+struct QkArgs {          // norm and rotation of q and k, forward or backward
+  Rows q, k;             // inputs
+  Rows gq, gk;           // backward: gradients of the outputs
+  Rows oq, ok;           // outputs: y, or the gradients of q and k
+  RotaryArgs rot;
+  int B, H, Hkv, N;
+  int heads;             // heads a workgroup takes one after another (q's or k's, never both)
+  int blocks;            // backward: workgroups per chunk of heads
+  float* part;           // backward: fp32 partial weight gradients [chunk, blocks][D]
+  void* dwq;
+  void* dwk;
+  void* stream;
+};
+
+struct AppendArgs {
+  Rows q, k, v, oq;      // oq: the turned queries (q.data null: none)
+  RotaryArgs rot;
+  ::fa_paged_cache cache;
+  const int* past;
+  const int* fresh;      // new tokens of each sequence; null: N
+  int B, H, N, D;
+  int heads;             // query heads a workgroup takes one after another
+  void* stream;
+};
+
+struct PagedArgs {
+  Rows q, o;
+  ::fa_paged_cache cache;
+  const int* past;
+  const int* fresh;
+  float* lse;            // [B, H, N]; null: none
+  float* part;           // partial rows of a split, null: none
+  int B, H, N, D;
+  int nsplit;
+  float scale_log2;
+  void* stream;
+};
+
 // keys per dK/dV workgroup (4 waves x 32 keys), for the split heuristics on the host
 constexpr int kDkdvKeys = 128;
 
 typedef int (*FwdFn)(const FwdArgs&);
 typedef int (*BwdFn)(const BwdArgs&);
+
+// (fa_rotary.hip, fa_paged.hip; arguments checked by fa_api.hip)
+int qk_norm_rotary(int dtype, int D, const QkArgs& a);
+int qk_norm_rotary_bwd(int dtype, int D, const QkArgs& a);
+size_t qk_norm_rotary_workspace(int B, int H, int Hkv, int N, int D);
+int paged_append(int dtype, const AppendArgs& a);
+int paged_attention(int dtype, PagedArgs a, size_t workspace_bytes);
+size_t paged_attention_workspace(int B, int H, int Hkv, int N, int D, long long keys);
 
 // Raise the dynamic LDS limit of a kernel once (needed above 64 KB).  The
 // static local makes the first call per kernel instance thread-safe.

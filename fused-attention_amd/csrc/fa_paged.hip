@@ -1,0 +1,480 @@
+// fa_paged.hip - keys and values in pages of 8-bit values with a scale for each page and head:
+// the append (norm, rotation, quantisation) and the attention over the pages, for gfx950.
+//
+// A value of a page is code 2^e, code an e4m3 number and 2^e the scale of its page and K/V head.
+// e4m3 is a floating format, so a scale only has to bring the page's largest value into range; with
+// powers of two it costs no rounding of its own, growing one moves the codes exactly (but for
+// subnormals), and both products below take it in exponent arithmetic.
+#include "fa_rotary.h"
+
+#include <algorithm>
+
+namespace fa {
+
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+
+constexpr int kScaleMin = -40, kScaleMax = 40;   // see attend: l needs the spread to stay far inside fp32's
+constexpr float kCodeMax = 448.f;
+
+__device__ __forceinline__ float exp2i(int e) { return __int_as_float((e + 127) << 23); }
+
+// The least e with amax <= 448 2^e (448 = 1.75 2^8), kept within the scales' range.
+__device__ __forceinline__ int scale_exponent(float amax) {
+  const uint32_t b = __float_as_uint(amax);
+  const int e = (int)(b >> 23) - 127 - 8 + ((b & 0x7FFFFFu) > 0x600000u ? 1 : 0);
+  return min(max(e, kScaleMin), kScaleMax);
+}
+
+// 8 values times `mul` as e4m3, to nearest even; past 448 to 448, infinities and NaN to NaN.
+__device__ __forceinline__ u32x2 encode8(const float (&y)[8], float mul) {
+  float z[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float x = y[i] * mul;
+    z[i] = __builtin_fabsf(y[i]) < __builtin_inff() ? __builtin_amdgcn_fmed3f(x, -kCodeMax, kCodeMax) : __builtin_nanf("");
+  }
+  u32x2 r;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    int w = 0;
+    w = __builtin_amdgcn_cvt_pk_fp8_f32(z[4 * i], z[4 * i + 1], w, false);
+    w = __builtin_amdgcn_cvt_pk_fp8_f32(z[4 * i + 2], z[4 * i + 3], w, true);
+    r[i] = (uint32_t)w;
+  }
+  return r;
+}
+
+__device__ __forceinline__ void decode8(const u32x2& w, float (&y)[8]) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[i], false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[i], true);
+    y[4 * i] = a[0], y[4 * i + 1] = a[1], y[4 * i + 2] = b[0], y[4 * i + 3] = b[1];
+  }
+}
+
+// The page that the table names for column `col` of sequence b; -1: none.
+__device__ __forceinline__ int page_of(const fa_paged_cache& c, int b, int col) {
+  if (col >= c.table_width) return -1;
+  const int p = c.block_table[b * c.table_stride + col];
+  return p >= 0 && p < c.num_pages ? p : -1;
+}
+
+// Lengths as the kernels use them: nothing negative, no sum past 31 bits.
+__device__ __forceinline__ int past_of(const int* past, int b) { return min(max(past[b], 0), 0x3FFFFFFF); }
+__device__ __forceinline__ int fresh_of(const int* fresh, int b, int N) { return fresh ? min(max(fresh[b], 0), N) : N; }
+
+// ---------------------------------------------------------------------------
+// Append.  The first q_blocks workgroups turn the queries (turn_heads); each of the others owns one
+// page of one sequence and K/V head, for K or for V, so nobody else writes its codes and scale: it
+// holds the page's new rows in registers, reduces their largest value, and writes codes. PASSES: rows
+// of a page over the rows that the workgroup holds at once.
+template <typename E, int D, bool INTER, int PASSES>
+__global__ __launch_bounds__(kRowThreads) void append_kernel(AppendArgs a, int q_blocks, int q_chunks, int touched) {
+  using S = Slot<D>;
+  const int slot = threadIdx.x / S::TPR;
+  const int Hkv = a.cache.H_kv, ps = a.cache.page_size;
+  if ((int)blockIdx.x < q_blocks) {
+    const int chunk = blockIdx.x % q_chunks;
+    const long long at = (long long)(blockIdx.x / q_chunks) * S::TOKENS + slot;
+    const bool valid = at < a.B * a.N;
+    const int t = valid ? (int)at : 0;
+    const int b = t / a.N, n = t % a.N, h0 = chunk * a.heads;
+    turn_heads<E, D, INTER>(a.rot, a.rot.q_weight, a.q, a.oq, b, n, (long long)past_of(a.past, b) + n, h0,
+                            min(h0 + a.heads, a.H), valid);
+    return;
+  }
+  int item = blockIdx.x - q_blocks;
+  const int h = item % Hkv;
+  item /= Hkv;
+  const bool is_k = item % 2 == 0;
+  item /= 2;
+  const int b = item / touched;
+  const int past = past_of(a.past, b), fresh = fresh_of(a.fresh, b, a.N);
+  const int col = past / ps + item % touched;
+  const int first = col * ps;                      // the page's first key
+  if (first >= past + fresh) return;
+  const int page = page_of(a.cache, b, col);
+  if (page < 0) return;
+  const int held = max(past - first, 0);           // rows the page holds already
+
+  const int lane = threadIdx.x & 63;
+  const int d0 = (threadIdx.x % S::TPR) * 8;
+  const long long ph = (long long)page * Hkv + h;
+  uint8_t* const codes = static_cast<uint8_t*>(is_k ? a.cache.k : a.cache.v) + ph * ps * D + d0;
+  uint8_t* const scale = static_cast<uint8_t*>(is_k ? a.cache.k_scale : a.cache.v_scale) + ph;
+  const int e_held = (int)*scale - 127;
+  const Rows& in = is_k ? a.k : a.v;
+  const uint16_t* src = static_cast<const uint16_t*>(in.data) + b * in.stride_b + h * in.stride_h + d0;
+
+  float y[PASSES][8];
+  float amax = 0.f;
+#pragma unroll
+  for (int p = 0; p < PASSES; ++p) {
+    const int n = first + p * S::TOKENS + slot - past;
+    const bool live = p * S::TOKENS + slot < ps && n >= 0 && n < fresh;
+    const int nn = live ? n : 0;
+    const u32x4 w = gload16(src + nn * in.stride_n);
+    if (is_k) {
+      Turn<D, INTER> turn;
+      turn.load(a.rot, lane, d0, b, nn, (long long)past + nn);
+      float cw[8], sw[8];
+      fold_weight<INTER>(turn.c, turn.s, a.rot, a.rot.k_weight, d0, cw, sw);
+      turn_row<E, D, INTER>(w, turn.fetch(w), cw, sw, a.rot.k_weight != nullptr, a.rot.eps, y[p]);
+    } else {
+      unpack8<E>(w, y[p]);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float x = __builtin_fabsf(y[p][i]);
+      if (live && x < __builtin_inff()) amax = fmaxf(amax, x);
+    }
+  }
+#pragma unroll
+  for (int m = 1; m < 64; m *= 2) amax = fmaxf(amax, __shfl_xor(amax, m));
+  __shared__ float top[kRowThreads / 64];
+  if (lane == 0) top[threadIdx.x / 64] = amax;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kRowThreads / 64; ++i) amax = fmaxf(amax, top[i]);
+  int e = scale_exponent(amax);
+  if (held > 0) e = max(e, e_held);
+  const float mul = exp2i(-e);
+#pragma unroll
+  for (int p = 0; p < PASSES; ++p) {
+    const int row = p * S::TOKENS + slot, n = first + row - past;
+    if (row < ps && n >= 0 && n < fresh) *reinterpret_cast<u32x2*>(codes + row * D) = encode8(y[p], mul);
+  }
+  if (held > 0 && e > e_held) {
+    const float move = __builtin_ldexpf(1.f, max(e_held - e, -100));
+    for (int row = slot; row < held; row += S::TOKENS) {
+      float z[8];
+      decode8(*reinterpret_cast<const u32x2*>(codes + row * D), z);
+      *reinterpret_cast<u32x2*>(codes + row * D) = encode8(z, move);
+    }
+  }
+  if (threadIdx.x == 0) *scale = (uint8_t)(e + 127);
+}
+
+// ---------------------------------------------------------------------------
+// Attention over the pages.
+//
+//   s'_ij = (q_i . code_j) c 2^ke(page) + ve(page),  c = log2(e) / sqrt(D)
+//   p'_ij = 2^(s'_ij - m'),  acc_i = sum_j p'_ij vcode_j,  l_i = sum_j 2^-ve p'_ij,  o = acc / l
+//
+// The V scale sits in the exponent: p' is measured by what its key adds to the output, so its
+// rounding to 16 bits (fp16: 2^-11 relative, next to the largest contribution) is safe for any mix of
+// scales, one accumulator serves all pages, and l, in fp32, takes the scales out again.  (|ve| <= 40 keeps
+// 2^-ve p' of every key that counts inside fp32's normal range.)  The codes go into the products
+// unscaled, exact in both 16-bit types: QK in the queries' type, PV in fp16.  m' is lazy and low: it
+// moves, to 7 below the largest score, when a score passes it by more than 15.  So p' <= 2^15, and
+// the many small weights of a long flat tail stay above fp16's subnormals down to 2^-21 of the largest.
+//
+// Rows: the N x G queries of a K/V head (G = H / H_kv), row r = token r / G, head r % G: 16 to a
+// workgroup, so each key's bytes serve all of them.  S^T = K Q^T as 16x16x32 products (16 keys x 16
+// rows): a lane owns one row, and the scores are fed back as the B operand of O^T += V^T P^T.  Two
+// 16-key tiles fill its 32 contraction slots; with slot (group g, j) = key 16 (j / 4) + 4 g + j % 4
+// no score moves between lanes, and V is read in that order, straight from the pages' rows: a lane
+// takes D / 16 dims of each of its 8 keys and pairs them up in registers.  Nothing is staged in LDS.
+constexpr int kWaves = 4;
+constexpr int kRows = 16;
+constexpr int kStep = 32;   // keys per step of a wave
+constexpr float kLazy = 15.f, kBelow = 7.f;
+
+__device__ __forceinline__ uint32_t cvt_f16(uint32_t w, bool hi) {
+  const f16x2 r = hi ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.f, true) : __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.f, false);
+  return __builtin_bit_cast(uint32_t, r);
+}
+
+template <typename E>
+__device__ __forceinline__ u32x4 codes8(uint32_t w0, uint32_t w1) {
+  if constexpr (std::is_same<E, F16>::value) {
+    return u32x4{cvt_f16(w0, false), cvt_f16(w0, true), cvt_f16(w1, false), cvt_f16(w1, true)};
+  } else {
+    return u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w0, 1.f, false)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w0, 1.f, true)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w1, 1.f, false)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w1, 1.f, true))};
+  }
+}
+
+// Any byte of w a NaN code (0x7F, 0xFF)?
+__device__ __forceinline__ bool has_nan(uint32_t w) { return (((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u) != 0; }
+
+// Over the four 16-lane groups of a wave.
+__device__ __forceinline__ float groups_max(float x) {
+  x = halfwave_max(x);
+  auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float groups_sum(float x) {
+  x = halfwave_sum(x);
+  auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+template <typename E, int D>
+__global__ __launch_bounds__(64 * kWaves) void attend_kernel(PagedArgs a, int row_blocks) {
+  constexpr int KB = D / 4;          // bytes of a K row per lane
+  constexpr int VB = D / 16;         // bytes of a V row per lane = 16-row blocks of O^T
+  constexpr int KT = D / 32;         // contraction steps over D
+  constexpr int KW = KB / 4;         // words
+  constexpr int LD = D + 4;          // row of the merge buffer
+  const float NEG_INF = -__builtin_inff();
+  __shared__ __attribute__((aligned(16))) float merge[kWaves][kRows][LD];
+  __shared__ float ml[kWaves][2][kRows];
+
+  const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int Hkv = a.cache.H_kv, ps = a.cache.page_size, G = a.H / Hkv;
+  const int rb = blockIdx.x % row_blocks, bh = blockIdx.x / row_blocks;
+  const int b = bh / Hkv, hk = bh % Hkv;
+  const int past = past_of(a.past, b), fresh = fresh_of(a.fresh, b, a.N);
+  const int r0 = rb * kRows, rows = a.N * G;
+  const int r = min(r0 + c, rows - 1), tok = r / G, head = hk * G + r % G;
+  const int lim = r0 + c < rows && tok < fresh ? past + tok : -1;    // last key this lane's row sees
+  const int tok0 = r0 / G, tok1 = min(min((r0 + kRows - 1) / G, a.N - 1), fresh - 1);
+  const int lmin = past + tok0;                                     // and the block's first live row
+  const int kend = tok0 < fresh ? past + tok1 + 1 : 0;              // keys that some row sees
+
+  // Q^T: column c, dims of step s: 64 (s / 2) + 16 g + 8 (s % 2) (D = 32: 8 g)
+  auto dim_of = [&](int s) __attribute__((always_inline)) { return D == 32 ? 8 * g : 64 * (s >> 1) + 16 * g + 8 * (s & 1); };
+  u32x4 qf[KT];
+  {
+    const uint16_t* q = static_cast<const uint16_t*>(a.q.data) + b * a.q.stride_b + head * a.q.stride_h + tok * a.q.stride_n;
+#pragma unroll
+    for (int s = 0; s < KT; ++s) qf[s] = gload16(q + dim_of(s));
+  }
+
+  f32x4 acc[VB];
+#pragma unroll
+  for (int x = 0; x < VB; ++x) acc[x] = f32x4{};
+  float m = -__FLT_MAX__, l = 0.f;
+
+  for (int k0 = wave * kStep; k0 < kend; k0 += kWaves * kStep) {
+    f32x4 s[2];
+    uint32_t vw[2][4][VB >= 4 ? VB / 4 : 1];
+    float ksc[2];
+    int ve[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int key = k0 + 16 * t;
+      const int page = key < kend ? page_of(a.cache, b, key / ps) : 0;
+      const long long ph = (long long)max(page, 0) * Hkv + hk;
+      ksc[t] = page < 0 ? __builtin_nanf("") : exp2i((int)static_cast<const uint8_t*>(a.cache.k_scale)[ph] - 127) * a.scale_log2;
+      ve[t] = page < 0 ? 0 : (int)static_cast<const uint8_t*>(a.cache.v_scale)[ph] - 127;
+      const long long off = (ph * ps + key % ps) * D;
+      const uint8_t* kp = static_cast<const uint8_t*>(a.cache.k) + off + c * D;
+      uint32_t kw[KW];
+      if constexpr (D == 32) {
+        const u32x2 w = *reinterpret_cast<const u32x2*>(kp + 8 * g);
+        kw[0] = w[0], kw[1] = w[1];
+      } else {
+#pragma unroll
+        for (int h = 0; h < D / 64; ++h) {
+          const u32x4 w = *reinterpret_cast<const u32x4*>(kp + 64 * h + 16 * g);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) kw[4 * h + j] = w[j];
+        }
+      }
+      const uint8_t* vp = static_cast<const uint8_t*>(a.cache.v) + off + 4 * g * D + c * VB;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (VB == 8) {
+          const u32x2 w = *reinterpret_cast<const u32x2*>(vp + i * D);
+          vw[t][i][0] = w[0], vw[t][i][1] = w[1];
+        } else if constexpr (VB == 4) {
+          vw[t][i][0] = *reinterpret_cast<const uint32_t*>(vp + i * D);
+        } else {
+          vw[t][i][0] = *reinterpret_cast<const uint16_t*>(vp + i * D);
+        }
+      }
+      s[t] = f32x4{};
+#pragma unroll
+      for (int u = 0; u < KT; ++u) s[t] = mfma16<E>(codes8<E>(kw[2 * u], kw[2 * u + 1]), qf[u], s[t]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[t][i] = __builtin_fmaf(s[t][i], ksc[t], (float)ve[t]);
+    }
+    const bool masked = k0 + kStep - 1 > lmin;
+    bool nan_v = false;
+    if (masked) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int key = k0 + 16 * t + 4 * g + i;
+          if (key > lim) s[t][i] = NEG_INF;
+#pragma unroll
+          for (int w = 0; w < (VB + 3) / 4; ++w) {
+            if (key >= kend) vw[t][i][w] = 0;       // what lies behind the last key may be anything
+            nan_v |= has_nan(vw[t][i][w]);
+          }
+        }
+    }
+    float mx = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
+                     fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+    mx = groups_max(mx);
+    if (__builtin_amdgcn_ballot_w64(mx > m + kLazy)) {
+      const float mn = fmaxf(m, mx - kBelow);
+      const float alpha = fast_exp2(m - mn);
+      m = mn;
+      l *= alpha;
+#pragma unroll
+      for (int x = 0; x < VB; ++x) acc[x] *= alpha;
+    }
+    float p[2][4];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) p[t][i] = fast_exp2(s[t][i] - m);
+      l = __builtin_fmaf((p[t][0] + p[t][1]) + (p[t][2] + p[t][3]), exp2i(-ve[t]), l);
+    }
+    // V^T operand of dims block x: slots j = 4 t + i are keys (t, i), the lane's dim c VB + x
+    auto v_operand = [&](int x) __attribute__((always_inline)) {
+      u32x4 r;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const uint32_t lo = cvt_f16(vw[w >> 1][2 * (w & 1)][x >> 2], (x & 2) != 0);
+        const uint32_t hi = cvt_f16(vw[w >> 1][2 * (w & 1) + 1][x >> 2], (x & 2) != 0);
+        r[w] = __builtin_amdgcn_perm(hi, lo, x & 1 ? 0x07060302u : 0x05040100u);
+      }
+      return r;
+    };
+    const u32x4 pf = {pack2<F16>(p[0][0], p[0][1]), pack2<F16>(p[0][2], p[0][3]), pack2<F16>(p[1][0], p[1][1]),
+                      pack2<F16>(p[1][2], p[1][3])};
+    if (__builtin_amdgcn_ballot_w64(nan_v)) {
+      // A NaN in V may lie behind some row's last key, where 0 NaN would reach that row: add the
+      // other values, then make NaN what sees one: counts = seen (1 or 0) x is NaN (1 or 0).
+      u32x4 seen;
+#pragma unroll
+      for (int w = 0; w < 4; ++w)
+        seen[w] = pack2<F16>(s[w >> 1][2 * (w & 1)] == NEG_INF ? 0.f : 1.f, s[w >> 1][2 * (w & 1) + 1] == NEG_INF ? 0.f : 1.f);
+#pragma unroll
+      for (int x = 0; x < VB; ++x) {
+        u32x4 v = v_operand(x), is;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const bool lo = (v[w] & 0x7FFFu) > 0x7C00u, hi = (v[w] & 0x7FFF0000u) > 0x7C000000u;
+          is[w] = (lo ? 0x3C00u : 0u) | (hi ? 0x3C000000u : 0u);
+          v[w] = (lo ? 0u : v[w] & 0xFFFFu) | (hi ? 0u : v[w] & 0xFFFF0000u);
+        }
+        acc[x] = mfma16<F16>(v, pf, acc[x]);
+        const f32x4 count = mfma16<F16>(is, seen, f32x4{});
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (count[i] > 0.f) acc[x][i] = __builtin_nanf("");
+      }
+    } else {
+#pragma unroll
+      for (int x = 0; x < VB; ++x) acc[x] = mfma16<F16>(v_operand(x), pf, acc[x]);
+    }
+  }
+
+  // merge of the waves: lane (c, g) holds row c, dims 4 g VB .. + 4 VB - 1
+  l = groups_sum(l);
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int x = 0; x < VB; ++x) merge[wave][c][(4 * g + i) * VB + x] = acc[x][i];
+  if (g == 0) ml[wave][0][c] = m, ml[wave][1][c] = l;
+  __syncthreads();
+  constexpr int PER = kRows * D / (64 * kWaves);   // values per thread (D = 32: 2)
+  constexpr int TR = D / PER;                      // threads per row
+  const int row = threadIdx.x / TR, d0 = threadIdx.x % TR * PER;
+  const int rr = r0 + row;
+  if (rr >= rows) return;
+  const int ot = rr / G, oh = hk * G + rr % G;
+  float M = -__FLT_MAX__, f[kWaves], L = 0.f, o[PER];
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) M = fmaxf(M, ml[w][0][row]);
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    f[w] = fast_exp2(ml[w][0][row] - M);
+    L = __builtin_fmaf(f[w], ml[w][1][row], L);
+  }
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    float x = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) x = __builtin_fmaf(f[w], merge[w][row][d0 + i], x);
+    o[i] = x;
+  }
+  const bool live = ot < fresh;
+  const float inv = live ? 1.0f / L : 0.f;
+  uint16_t* dst = static_cast<uint16_t*>(const_cast<void*>(a.o.data)) + b * a.o.stride_b + oh * a.o.stride_h + ot * a.o.stride_n + d0;
+#pragma unroll
+  for (int i = 0; i < PER; i += 2)
+    *reinterpret_cast<uint32_t*>(dst + i) = live ? pack2<E>(o[i] * inv, o[i + 1] * inv) : 0u;
+  if (a.lse != nullptr && d0 == 0) a.lse[((long long)b * a.H + oh) * a.N + ot] = live ? M + __log2f(L) : NEG_INF;
+}
+
+// ---------------------------------------------------------------------------
+namespace {
+
+template <typename E, int D, bool INTER>
+int launch_append_passes(const AppendArgs& a, int q_blocks, int q_chunks, int touched, long long grid) {
+  const dim3 g((unsigned)grid), t(kRowThreads);
+  hipStream_t st = (hipStream_t)a.stream;
+  const int passes = std::max(1, a.cache.page_size / Slot<D>::TOKENS);
+  if (passes == 1) hipLaunchKernelGGL((append_kernel<E, D, INTER, 1>), g, t, 0, st, a, q_blocks, q_chunks, touched);
+  else if (passes == 2) hipLaunchKernelGGL((append_kernel<E, D, INTER, 2>), g, t, 0, st, a, q_blocks, q_chunks, touched);
+  else if constexpr (D >= 64) {
+    if (passes == 4) hipLaunchKernelGGL((append_kernel<E, D, INTER, 4>), g, t, 0, st, a, q_blocks, q_chunks, touched);
+    else if constexpr (D >= 128) hipLaunchKernelGGL((append_kernel<E, D, INTER, 8>), g, t, 0, st, a, q_blocks, q_chunks, touched);
+  }
+  return hipGetLastError() == hipSuccess ? FA_OK : FA_ERR_LAUNCH;
+}
+
+template <typename E, int D>
+int launch_append(AppendArgs a) {
+  const int ps = a.cache.page_size, touched = (a.N + ps - 2) / ps + 1;
+  const long long items = 2LL * a.B * touched * a.cache.H_kv;
+  long long q_blocks = 0;
+  int q_chunks = 0;
+  if (a.q.data != nullptr) {
+    const long long token_blocks = ((long long)a.B * a.N + Slot<D>::TOKENS - 1) / Slot<D>::TOKENS;
+    a.heads = 8;
+    while (a.heads > 1 && token_blocks * ((a.H + a.heads - 1) / a.heads) < 2LL * cu_count()) a.heads /= 2;
+    q_chunks = (a.H + a.heads - 1) / a.heads;
+    q_blocks = token_blocks * q_chunks;
+  }
+  if (items + q_blocks > 0x7fffffffLL) return FA_ERR_DIMS;
+  return a.rot.interleaved ? launch_append_passes<E, D, true>(a, (int)q_blocks, q_chunks, touched, items + q_blocks)
+                           : launch_append_passes<E, D, false>(a, (int)q_blocks, q_chunks, touched, items + q_blocks);
+}
+
+template <typename E, int D>
+int launch_attend(const PagedArgs& a) {
+  const int rows = a.N * (a.H / a.cache.H_kv), row_blocks = (rows + kRows - 1) / kRows;
+  const long long grid = (long long)a.B * a.cache.H_kv * row_blocks;
+  if (grid > 0x7fffffffLL) return FA_ERR_DIMS;
+  hipLaunchKernelGGL((attend_kernel<E, D>), dim3((unsigned)grid), dim3(64 * kWaves), 0, (hipStream_t)a.stream, a, row_blocks);
+  return hipGetLastError() == hipSuccess ? FA_OK : FA_ERR_LAUNCH;
+}
+
+}  // namespace
+
+int paged_append(int dtype, const AppendArgs& a) {
+  if (dtype == FA_BF16) {
+    if (a.D == 32) return launch_append<BF16, 32>(a);
+    if (a.D == 64) return launch_append<BF16, 64>(a);
+    return launch_append<BF16, 128>(a);
+  }
+  if (a.D == 32) return launch_append<F16, 32>(a);
+  if (a.D == 64) return launch_append<F16, 64>(a);
+  return launch_append<F16, 128>(a);
+}
+
+int paged_attention(int dtype, PagedArgs a, size_t) {
+  if (dtype == FA_BF16) {
+    if (a.D == 32) return launch_attend<BF16, 32>(a);
+    if (a.D == 64) return launch_attend<BF16, 64>(a);
+    return launch_attend<BF16, 128>(a);
+  }
+  if (a.D == 32) return launch_attend<F16, 32>(a);
+  if (a.D == 64) return launch_attend<F16, 64>(a);
+  return launch_attend<F16, 128>(a);
+}
+
+size_t paged_attention_workspace(int, int, int, int, int, long long) { return 0; }
+
+}  // namespace fa

@@ -1,0 +1,219 @@
+// fa_rotary.h - norm and position rotation of one row (one head of one token), the part that the
+// rotary kernels (fa_rotary.hip) and the paged cache's append (fa_paged.hip) share.
+//
+//   y = R(p) (w o x r),  r = (mean(x^2) + eps)^(-1/2)
+//
+// R(p) turns pairs of the first `rotary` dims: (a, b) -> (a cos - b sin, b cos + a sin), the cosine
+// and sine read from a table row of the pair's position; pair j is dims (j, j + rotary / 2), or
+// (2j, 2j + 1) when interleaved; dims past `rotary` keep their normed value.
+//
+// A row of D values is held by a team of D / 8 lanes, 8 consecutive dims (16 bytes) each.  With
+// `rotary` a multiple of 16, a lane's 8 dims lie in one half of the rotated part, so its partners
+// are the 8 dims of one other lane (or its own, interleaved): y = r (x (C w) + x_partner (S w_partner)),
+// with the partner's values moved as the row's packed 16-bit words, 4 moves instead of 8.
+#pragma once
+
+#include "fa_device.h"
+#include "fa_launch.h"
+
+namespace fa {
+
+// 8 packed 16-bit values as fp32.
+template <typename E>
+__device__ __forceinline__ void unpack8(const u32x4& w, float (&x)[8]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    x[2 * i] = to_f32<E>(w[i] & 0xFFFFu);
+    x[2 * i + 1] = to_f32<E>(w[i] >> 16);
+  }
+}
+
+template <typename E>
+__device__ __forceinline__ u32x4 pack8(const float (&x)[8]) {
+  return u32x4{pack2<E>(x[0], x[1]), pack2<E>(x[2], x[3]), pack2<E>(x[4], x[5]), pack2<E>(x[6], x[7])};
+}
+
+// Sum over the T lanes of a team (T = 4, 8 or 16 neighbours).
+template <int T>
+__device__ __forceinline__ float team_sum(float x) {
+  x = quad_sum(x);
+  // DPP row_half_mirror / row_mirror: lanes of one quad hold the same sum by then
+  if constexpr (T >= 8) x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x141, 0xF, 0xF, false));
+  if constexpr (T >= 16) x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x140, 0xF, 0xF, false));
+  return x;
+}
+
+// What a lane needs to turn the rows of one token.
+template <int D, bool INTER>
+struct Turn {
+  float c[8], s[8];  // own value's factor; partner's factor, with its sign
+  int partner;       // lane that holds the partners (interleaved: none)
+
+  __device__ __forceinline__ static int partner_lane(const RotaryArgs& a, int lane, int d0) {
+    if (INTER || d0 >= a.rotary_dim) return lane;
+    const int half = a.rotary_dim / 2;
+    return d0 < half ? lane + half / 8 : lane - half / 8;
+  }
+
+  // Position of a pair: its axis by the sections, the token's entry of that axis.  `base`: the
+  // position when no positions are given.
+  __device__ __forceinline__ static long long position(const RotaryArgs& a, int pair, int b, int n, long long base) {
+    if (a.positions == nullptr) return base;
+    int axis = 0;
+#pragma unroll
+    for (int i = 0; i < kMaxAxes - 1; ++i) axis += i < a.axes - 1 && pair >= a.section_end[i] ? 1 : 0;
+    const long long at = axis * a.pos_axis_stride + (long long)b * a.pos_batch_stride + n;
+    return a.positions_int64 ? static_cast<const long long*>(a.positions)[at] : static_cast<const int*>(a.positions)[at];
+  }
+
+  // Factors of token (b, n) for dims d0 .. d0 + 7.  A negative position leaves the row unturned
+  // (padding); one past the table gives NaN.
+  __device__ __forceinline__ void load(const RotaryArgs& a, int lane, int d0, int b, int n, long long base) {
+    partner = partner_lane(a, lane, d0);
+    const bool turned = a.table != nullptr && d0 < a.rotary_dim;
+    if (!turned) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) c[i] = 1.f, s[i] = 0.f;
+      return;
+    }
+    const int half = a.rotary_dim / 2;
+    constexpr int NP = INTER ? 4 : 8;   // pairs of this lane
+    const int pair0 = INTER ? d0 / 2 : (d0 < half ? d0 : d0 - half);
+    float cc[NP], ss[NP];
+    if (a.axes == 1) {
+      const long long p = position(a, 0, b, n, base);
+      const float* row = a.table + (p < 0 ? 0 : p >= a.table_len ? 0 : p) * a.rotary_dim + pair0;
+#pragma unroll
+      for (int i = 0; i < NP; i += 4) {
+        const f32x4 x = gload_f32x4(row + i), y = gload_f32x4(row + half + i);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) cc[i + j] = x[j], ss[i + j] = y[j];
+      }
+      const float bad = p >= a.table_len ? __builtin_nanf("") : 0.f;
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+        cc[i] = p < 0 ? 1.f : cc[i] + bad;
+        ss[i] = p < 0 ? 0.f : ss[i] + bad;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+        const long long p = position(a, pair0 + i, b, n, base);
+        const bool in = p >= 0 && p < a.table_len;
+        const float* row = a.table + (in ? p : 0) * a.rotary_dim + pair0 + i;
+        const float x = row[0], y = row[half];
+        cc[i] = in ? x : p < 0 ? 1.f : __builtin_nanf("");
+        ss[i] = in ? y : p < 0 ? 0.f : __builtin_nanf("");
+      }
+    }
+    if constexpr (INTER) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        c[2 * i] = c[2 * i + 1] = cc[i];
+        s[2 * i] = -ss[i];
+        s[2 * i + 1] = ss[i];
+      }
+    } else {
+      const float sign = d0 < half ? -1.f : 1.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) c[i] = cc[i], s[i] = sign * ss[i];
+    }
+  }
+
+  // The partner lane's packed row (its own when interleaved: the pairs are inside the lane).
+  __device__ __forceinline__ u32x4 fetch(const u32x4& w) const {
+    if constexpr (INTER) return w;
+    u32x4 r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = (uint32_t)__builtin_amdgcn_ds_bpermute(partner << 2, (int)w[i]);
+    return r;
+  }
+};
+
+// Partner's value of dim i out of the values that fetch() brought.
+template <bool INTER>
+__device__ __forceinline__ float partner_of(const float (&xp)[8], int i) {
+  return INTER ? xp[i ^ 1] : xp[i];
+}
+
+// Norm weight of dims d0 .. d0 + 7 (ones without one).
+__device__ __forceinline__ void load_weight(const RotaryArgs& a, const void* w, int d0, float (&x)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    if (w == nullptr) x[i] = 1.f;
+    else if (a.weight_dtype == FA_F32) x[i] = static_cast<const float*>(w)[d0 + i];
+    else if (a.weight_dtype == FA_BF16) x[i] = to_f32<BF16>(static_cast<const uint16_t*>(w)[d0 + i]);
+    else x[i] = to_f32<F16>(static_cast<const uint16_t*>(w)[d0 + i]);
+  }
+}
+
+template <int D>
+__device__ __forceinline__ float inv_rms(const float (&x)[8], float eps) {
+  float ss = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) ss = __builtin_fmaf(x[i], x[i], ss);
+  return 1.0f / __builtin_sqrtf(team_sum<D / 8>(ss) * (1.0f / D) + eps);
+}
+
+// One row: x packed (and its partner's), cw = C w and sw = S w_partner of its token and tensor.
+template <typename E, int D, bool INTER>
+__device__ __forceinline__ void turn_row(const u32x4& w, const u32x4& wp, const float (&cw)[8], const float (&sw)[8],
+                                         bool norm, float eps, float (&y)[8]) {
+  float x[8], xp[8];
+  unpack8<E>(w, x);
+  unpack8<E>(wp, xp);
+  const float r = norm ? inv_rms<D>(x, eps) : 1.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) y[i] = r * __builtin_fmaf(x[i], cw[i], partner_of<INTER>(xp, i) * sw[i]);
+}
+
+template <bool INTER>
+__device__ __forceinline__ void fold_weight(const float (&c)[8], const float (&s)[8], const RotaryArgs& a, const void* w,
+                                            int d0, float (&cw)[8], float (&sw)[8]) {
+  float own[8], other[8];
+  load_weight(a, w, d0, own);
+  const int half = a.rotary_dim / 2;
+  const bool turned = a.table != nullptr && d0 < a.rotary_dim;
+  load_weight(a, w, INTER || !turned ? d0 : d0 < half ? d0 + half : d0 - half, other);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    cw[i] = c[i] * own[i];
+    sw[i] = s[i] * partner_of<INTER>(other, i);
+  }
+}
+
+constexpr int kRowThreads = 256;
+constexpr int kRowBatch = 4;     // heads whose rows are in flight at a time
+
+template <int D>
+struct Slot {
+  static constexpr int TPR = D / 8;                 // lanes per row
+  static constexpr int TOKENS = kRowThreads / TPR;  // rows a workgroup holds at once
+};
+
+// Heads h0 .. h1 - 1 of token (b, n): one team of lanes, the heads one after another, the token's
+// table row and the weight folded into registers once.
+template <typename E, int D, bool INTER>
+__device__ __forceinline__ void turn_heads(const RotaryArgs& rot, const void* w, const Rows& in, const Rows& out, int b,
+                                           int n, long long base, int h0, int h1, bool valid) {
+  const int d0 = (threadIdx.x % Slot<D>::TPR) * 8;
+  Turn<D, INTER> turn;
+  turn.load(rot, threadIdx.x & 63, d0, b, n, base);
+  float cw[8], sw[8];
+  fold_weight<INTER>(turn.c, turn.s, rot, w, d0, cw, sw);
+  const uint16_t* src = static_cast<const uint16_t*>(in.data) + b * in.stride_b + n * in.stride_n + d0;
+  uint16_t* dst = static_cast<uint16_t*>(const_cast<void*>(out.data)) + b * out.stride_b + n * out.stride_n + d0;
+  for (int h = h0; h < h1; h += kRowBatch) {
+    u32x4 x[kRowBatch];
+#pragma unroll
+    for (int i = 0; i < kRowBatch; ++i) x[i] = gload16(src + min(h + i, h1 - 1) * in.stride_h);
+#pragma unroll
+    for (int i = 0; i < kRowBatch; ++i) {
+      float y[8];
+      turn_row<E, D, INTER>(x[i], turn.fetch(x[i]), cw, sw, w != nullptr, rot.eps, y);
+      if (valid && h + i < h1) gstore16(dst + (h + i) * out.stride_h, pack8<E>(y));
+    }
+  }
+}
+
+}  // namespace fa

@@ -28,7 +28,7 @@
 extern "C" {
 #endif
 
-enum fa_dtype { FA_F16 = 0, FA_BF16 = 1 };
+enum fa_dtype { FA_F16 = 0, FA_BF16 = 1, FA_F32 = 2 /* norm weights alone */ };
 
 enum fa_status {
   FA_OK = 0,
@@ -42,7 +42,10 @@ enum fa_status {
   FA_ERR_UNSUPPORTED = -7, /* valid arguments, but no kernel for this combination */
   FA_ERR_WORKSPACE = -8,   /* fa_bwd_gqa*: workspace not 16-byte aligned; fa_bwd_gqa_exact:
                               also a workspace too small for the requested split */
-  FA_ERR_SCRATCH = -9      /* fa_bwd_gqa_noalloc: the per-row terms exceed the library's scratch */
+  FA_ERR_SCRATCH = -9,     /* fa_bwd_gqa_noalloc: the per-row terms exceed the library's scratch */
+  FA_ERR_LAYOUT = -10,     /* fa_rows: data not 16-byte aligned, or a stride no multiple of 8 */
+  FA_ERR_ROTATION = -11,   /* fa_rotation: table, sections, weights or axes outside what it allows */
+  FA_ERR_PAGES = -12       /* fa_paged_cache: page size, counts, alignment or strides outside what it allows */
 };
 
 /*
@@ -203,6 +206,100 @@ FA_API int fa_bwd_dkdv_split(int B, int H, int H_kv, int S, int D);
  * per-row terms, plus the partial sums when the key tiles alone leave the GPU
  * idle (0 for invalid dimensions).  No reference counterpart. */
 FA_API size_t fa_bwd_gqa_workspace_size(int B, int H, int H_kv, int S, int D);
+
+/*
+ * Norm of queries and keys for each head, with the position rotation in the same pass, and its
+ * backward.  No counterpart in the reference, whose inputs are already normed and turned.
+ *
+ *   y = R(p) (w o x r),  r = (mean(x^2) + eps)^(-1/2) over the D values of a row (one head of one token)
+ *
+ * Rows are [B, heads, N, D], D contiguous, the other strides free (in elements, multiples of 8; data
+ * 16-byte aligned), so the views of a packed projection [B, N, heads, D] are read as they are.
+ * fa_rotation:
+ *   q_weight, k_weight : norm weights [D] of weight_dtype (the rows' type or FA_F32); NULL, both: no norm
+ *   table  : [table_len, rotary_dim] fp32, the cosines of the rotary_dim / 2 pairs, then their sines;
+ *            16-byte aligned; NULL: no rotation.  rotary_dim: a multiple of 16 up to D; dims past it keep
+ *            their normed value.  Pair j is dims (j, j + rotary_dim / 2), or (2j, 2j + 1) if interleaved.
+ *   positions : [axes, B, N] int32 (int64 with positions_int64), unit stride along N; NULL: token n is
+ *            at n (the append: past_lens[b] + n).  A negative position leaves its row unturned; one of
+ *            table_len or more gives NaN.
+ *   axes   : 1 to 3; pair j turns with the first axis a with j < section_end[a], else the last.
+ *
+ * fa_qk_norm_rotary writes q_out and k_out.
+ * fa_qk_norm_rotary_bwd: from the gradients gq, gk of the outputs, those of the inputs (dq, dk) and of
+ *   the weights (dwq, dwk, [D] of weight_dtype, summed in fp32 in a fixed order; NULL without a norm).
+ *   workspace: fa_qk_norm_rotary_workspace_size() bytes, 16-byte aligned (0: without a norm, none).
+ */
+typedef struct fa_rows {
+  const void* data;
+  long long stride_b, stride_h, stride_n;
+} fa_rows;
+
+typedef struct fa_rotation {
+  const float* table;
+  const void* positions;
+  const void* q_weight;
+  const void* k_weight;
+  long long pos_axis_stride, pos_batch_stride;
+  int table_len, rotary_dim, axes, positions_int64;
+  int section_end[2];
+  int weight_dtype, interleaved;
+  float eps;
+} fa_rotation;
+
+FA_API int fa_qk_norm_rotary(const fa_rows* q, const fa_rows* k, const fa_rows* q_out, const fa_rows* k_out,
+                      const fa_rotation* rotation, int B, int H, int H_kv, int N, int D, int dtype,
+                      void* hip_stream);
+FA_API int fa_qk_norm_rotary_bwd(const fa_rows* q, const fa_rows* k, const fa_rows* gq, const fa_rows* gk,
+                          const fa_rows* dq, const fa_rows* dk, void* dwq, void* dwk,
+                          const fa_rotation* rotation, int B, int H, int H_kv, int N, int D, int dtype,
+                          void* workspace, size_t workspace_bytes, void* hip_stream);
+FA_API size_t fa_qk_norm_rotary_workspace_size(int B, int H, int H_kv, int N, int D);
+
+/*
+ * Keys and values of many sequences held in pages of 8-bit values, with a scale for each page and
+ * head, and attention over them.  No counterpart in the reference.
+ *
+ * fa_paged_cache: k, v [num_pages, H_kv, page_size, D] e4m3 (OCP: 448 largest, no infinity), 16-byte
+ *   aligned; k_scale, v_scale [num_pages, H_kv], the scale 2^(byte - 127).  page_size 16, 32, 64 or
+ *   128.  block_table [B, table_width] int32 (row stride table_stride): the page of keys
+ *   [i page_size, (i + 1) page_size) of sequence b.
+ * past_lens [B] int32: tokens that a sequence held before this call's; new_lens [B]: this call's
+ *   (NULL: N each), the rest of the N being padding.  Values outside [0, N] count as the nearer bound.
+ *
+ * fa_paged_append stores token n of sequence b as key past_lens[b] + n: k normed and turned (fa_rotation,
+ *   with k_weight), v as it is, and, where q is given, writes q normed and turned (padding too) to q_out.
+ *   Scale of a page and head: the least power of two 2^e, -40 <= e <= 40, with |x| <= 448 2^e for its finite
+ *   values; a page whose first row is written starts anew, else e only grows, and the rows it holds are
+ *   moved along (exactly, but for values that become subnormal).  A finite value past 448 2^40 becomes
+ *   that, an infinity or NaN becomes NaN.  Rows behind the last new token keep their bytes.  A token whose page the table does not
+ *   name (out of [0, num_pages), or past table_width) is not stored.  Pages that are written must
+ *   belong to one sequence.
+ * fa_paged_attention: query n of sequence b against keys 0 .. past_lens[b] + n of its pages, scale 1/sqrt(D)
+ *   folded in scale_log2 as in fa_fwd; query head h reads K/V head h / (H / H_kv).  q, o: rows as above.
+ *   Padding gets zeros (lse -inf).  lse: NULL or [B, H, N] fp32 in fa_fwd's units.  A key whose page the
+ *   table does not name makes the rows that see it NaN.  What lies behind a row's last key does not
+ *   touch it, NaN included.
+ *   workspace: fa_paged_attention_workspace_size() bytes, 16-byte aligned, for the partial rows of keys
+ *   split over workgroups; with less (NULL) they are split less or not at all.
+ */
+typedef struct fa_paged_cache {
+  void* k;
+  void* v;
+  void* k_scale;
+  void* v_scale;
+  const int* block_table;
+  long long table_stride;
+  int table_width, num_pages, page_size, H_kv;
+} fa_paged_cache;
+
+FA_API int fa_paged_append(const fa_rows* q, const fa_rows* k, const fa_rows* v, const fa_rows* q_out,
+                    const fa_paged_cache* cache, const int* past_lens, const int* new_lens,
+                    const fa_rotation* rotation, int B, int H, int N, int D, int dtype, void* hip_stream);
+FA_API int fa_paged_attention(const fa_rows* q, const fa_paged_cache* cache, const int* past_lens,
+                       const int* new_lens, const fa_rows* o, float* lse, int B, int H, int N, int D,
+                       int dtype, float scale_log2, void* workspace, size_t workspace_bytes, void* hip_stream);
+FA_API size_t fa_paged_attention_workspace_size(int B, int H, int H_kv, int N, int D, long long keys);
 
 /* 1 if a forward (with_lse 0/1) or backward (is_bwd 1) kernel exists for the
  * combination, else 0.  No reference counterpart: it lets a caller probe the
