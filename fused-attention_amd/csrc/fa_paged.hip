@@ -212,12 +212,82 @@ __device__ __forceinline__ float groups_sum(float x) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
+// The keys of one 16-key tile of a wave: its K and V bytes in registers.
+template <int D>
+struct Tile {
+  static constexpr int KB = D / 4;    // bytes of a K row per lane
+  static constexpr int VB = D / 16;   // bytes of a V row per lane = 16-row blocks of O^T
+  static constexpr int VW = VB >= 4 ? VB / 4 : 1;
+  uint32_t k[KB / 4];
+  uint32_t v[4][VW];
+
+  // base: the tile's offset in the pools (uniform); lane (c, g): K row c, 16-byte pieces g of each 64;
+  // V rows 4 g + i, bytes c VB
+  __device__ __forceinline__ void load(const uint8_t* kp, const uint8_t* vp, long long base, int c, int g) {
+    const uint8_t* const k0 = kp + base;
+    const uint8_t* const v0 = vp + base;
+    if constexpr (D == 32) {
+      const u32x2 w = *reinterpret_cast<const u32x2*>(k0 + c * D + 8 * g);
+      k[0] = w[0], k[1] = w[1];
+    } else {
+#pragma unroll
+      for (int h = 0; h < D / 64; ++h) {
+        const u32x4 w = *reinterpret_cast<const u32x4*>(k0 + c * D + 64 * h + 16 * g);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) k[4 * h + j] = w[j];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint8_t* const p = v0 + (4 * g + i) * D + c * VB;
+      if constexpr (VB == 8) {
+        const u32x2 w = *reinterpret_cast<const u32x2*>(p);
+        v[i][0] = w[0], v[i][1] = w[1];
+      } else if constexpr (VB == 4) {
+        v[i][0] = *reinterpret_cast<const uint32_t*>(p);
+      } else {
+        v[i][0] = *reinterpret_cast<const uint16_t*>(p);
+      }
+    }
+  }
+};
+
+// Keys of a split of a row block: `keys` keys that some row sees in at most nsplit parts, each whole
+// steps of the workgroup's waves.
+__host__ __device__ __forceinline__ int split_keys(int keys, int nsplit) {
+  const int step = kWaves * kStep;
+  const int per = (keys + nsplit - 1) / nsplit;
+  return max((per + step - 1) / step * step, step);
+}
+
+// Token range of a row block, and how many keys its rows see.
+struct Block {
+  int past, fresh, r0, rows, lmin, keys;
+};
+
+__device__ __forceinline__ Block block_of(const PagedArgs& a, int b, int rb, int G) {
+  Block x;
+  x.past = past_of(a.past, b);
+  x.fresh = fresh_of(a.fresh, b, a.N);
+  x.r0 = rb * kRows;
+  x.rows = a.N * G;
+  const int tok0 = x.r0 / G, tok1 = min(min((x.r0 + kRows - 1) / G, a.N - 1), x.fresh - 1);
+  x.lmin = x.past + tok0;                              // the last key that the first live row sees
+  x.keys = tok0 < x.fresh ? x.past + tok1 + 1 : 0;
+  return x;
+}
+
+// A split leaves, for each row, D unnormalised sums, m' and l.
+template <int D>
+__device__ __forceinline__ float* part_row(const PagedArgs& a, long long block, int split, int row) {
+  return a.part + ((block * a.nsplit + split) * kRows + row) * (D + 4);
+}
+
 template <typename E, int D>
 __global__ __launch_bounds__(64 * kWaves) void attend_kernel(PagedArgs a, int row_blocks) {
-  constexpr int KB = D / 4;          // bytes of a K row per lane
-  constexpr int VB = D / 16;         // bytes of a V row per lane = 16-row blocks of O^T
+  typedef Tile<D> T;
+  constexpr int VB = T::VB;
   constexpr int KT = D / 32;         // contraction steps over D
-  constexpr int KW = KB / 4;         // words
   constexpr int LD = D + 4;          // row of the merge buffer
   const float NEG_INF = -__builtin_inff();
   __shared__ __attribute__((aligned(16))) float merge[kWaves][kRows][LD];
@@ -226,15 +296,17 @@ __global__ __launch_bounds__(64 * kWaves) void attend_kernel(PagedArgs a, int ro
   const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int Hkv = a.cache.H_kv, ps = a.cache.page_size, G = a.H / Hkv;
-  const int rb = blockIdx.x % row_blocks, bh = blockIdx.x / row_blocks;
+  const int split = blockIdx.x % a.nsplit;
+  const long long block = blockIdx.x / a.nsplit;
+  const int rb = block % row_blocks, bh = block / row_blocks;
   const int b = bh / Hkv, hk = bh % Hkv;
-  const int past = past_of(a.past, b), fresh = fresh_of(a.fresh, b, a.N);
-  const int r0 = rb * kRows, rows = a.N * G;
-  const int r = min(r0 + c, rows - 1), tok = r / G, head = hk * G + r % G;
-  const int lim = r0 + c < rows && tok < fresh ? past + tok : -1;    // last key this lane's row sees
-  const int tok0 = r0 / G, tok1 = min(min((r0 + kRows - 1) / G, a.N - 1), fresh - 1);
-  const int lmin = past + tok0;                                     // and the block's first live row
-  const int kend = tok0 < fresh ? past + tok1 + 1 : 0;              // keys that some row sees
+  const Block x = block_of(a, b, rb, G);
+  const int per = split_keys(x.keys, a.nsplit);
+  const int first = split * per, last = min(first + per, x.keys);   // keys of this workgroup
+  if (split > 0 && first >= x.keys) return;                        // (the first split also writes what has no keys)
+
+  const int r = min(x.r0 + c, x.rows - 1), tok = r / G, head = hk * G + r % G;
+  const int lim = x.r0 + c < x.rows && tok < x.fresh ? x.past + tok : -1;    // last key this lane's row sees
 
   // Q^T: column c, dims of step s: 64 (s / 2) + 16 g + 8 (s % 2) (D = 32: 8 g)
   auto dim_of = [&](int s) __attribute__((always_inline)) { return D == 32 ? 8 * g : 64 * (s >> 1) + 16 * g + 8 * (s & 1); };
@@ -247,66 +319,56 @@ __global__ __launch_bounds__(64 * kWaves) void attend_kernel(PagedArgs a, int ro
 
   f32x4 acc[VB];
 #pragma unroll
-  for (int x = 0; x < VB; ++x) acc[x] = f32x4{};
+  for (int i = 0; i < VB; ++i) acc[i] = f32x4{};
   float m = -__FLT_MAX__, l = 0.f;
+  const uint8_t* const kp = static_cast<const uint8_t*>(a.cache.k);
+  const uint8_t* const vp = static_cast<const uint8_t*>(a.cache.v);
 
-  for (int k0 = wave * kStep; k0 < kend; k0 += kWaves * kStep) {
+  // Step j of this wave: keys first + (4 j + wave) 32 + 0..31, two tiles.  Lane i keeps page and scales of
+  // its wave's tile i of a run of 32 steps, so the loop below waits for no address.
+  const int steps = last > first ? (last - first + kWaves * kStep - 1) / (kWaves * kStep) : 0;
+  int my_page = 0, my_ve = 0, my_row = 0;
+  float my_ks = 0.f;
+  auto load_run = [&](int j0) __attribute__((always_inline)) {
+    const int key = first + ((j0 + lane / 2) * kWaves + wave) * kStep + 16 * (lane & 1);
+    int page = key < last ? page_of(a.cache, b, key / ps) : 0;
+    const long long ph = (long long)max(page, 0) * Hkv + hk;
+    const int ke = static_cast<const uint8_t*>(a.cache.k_scale)[ph], ve = static_cast<const uint8_t*>(a.cache.v_scale)[ph];
+    my_ks = page < 0 ? __builtin_nanf("") : exp2i(ke - 127) * a.scale_log2;   // (no page: its rows become NaN)
+    my_ve = page < 0 ? 0 : ve - 127;
+    my_page = max(page, 0);
+    my_row = key % ps;
+  };
+  auto load_tile = [&](T& t, int i) __attribute__((always_inline)) {   // tile i of the run
+    const int page = __builtin_amdgcn_readlane(my_page, i), row = __builtin_amdgcn_readlane(my_row, i);
+    t.load(kp, vp, (((long long)page * Hkv + hk) * ps + row) * D, c, g);
+  };
+
+  auto compute = [&](T (&t)[2], int i, int k0) __attribute__((always_inline)) {
     f32x4 s[2];
-    uint32_t vw[2][4][VB >= 4 ? VB / 4 : 1];
-    float ksc[2];
     int ve[2];
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const int key = k0 + 16 * t;
-      const int page = key < kend ? page_of(a.cache, b, key / ps) : 0;
-      const long long ph = (long long)max(page, 0) * Hkv + hk;
-      ksc[t] = page < 0 ? __builtin_nanf("") : exp2i((int)static_cast<const uint8_t*>(a.cache.k_scale)[ph] - 127) * a.scale_log2;
-      ve[t] = page < 0 ? 0 : (int)static_cast<const uint8_t*>(a.cache.v_scale)[ph] - 127;
-      const long long off = (ph * ps + key % ps) * D;
-      const uint8_t* kp = static_cast<const uint8_t*>(a.cache.k) + off + c * D;
-      uint32_t kw[KW];
-      if constexpr (D == 32) {
-        const u32x2 w = *reinterpret_cast<const u32x2*>(kp + 8 * g);
-        kw[0] = w[0], kw[1] = w[1];
-      } else {
+    for (int u = 0; u < 2; ++u) {
+      const float ks = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(my_ks), i + u));
+      ve[u] = __builtin_amdgcn_readlane(my_ve, i + u);
+      s[u] = f32x4{};
 #pragma unroll
-        for (int h = 0; h < D / 64; ++h) {
-          const u32x4 w = *reinterpret_cast<const u32x4*>(kp + 64 * h + 16 * g);
+      for (int n = 0; n < KT; ++n) s[u] = mfma16<E>(codes8<E>(t[u].k[2 * n], t[u].k[2 * n + 1]), qf[n], s[u]);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) kw[4 * h + j] = w[j];
-        }
-      }
-      const uint8_t* vp = static_cast<const uint8_t*>(a.cache.v) + off + 4 * g * D + c * VB;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if constexpr (VB == 8) {
-          const u32x2 w = *reinterpret_cast<const u32x2*>(vp + i * D);
-          vw[t][i][0] = w[0], vw[t][i][1] = w[1];
-        } else if constexpr (VB == 4) {
-          vw[t][i][0] = *reinterpret_cast<const uint32_t*>(vp + i * D);
-        } else {
-          vw[t][i][0] = *reinterpret_cast<const uint16_t*>(vp + i * D);
-        }
-      }
-      s[t] = f32x4{};
-#pragma unroll
-      for (int u = 0; u < KT; ++u) s[t] = mfma16<E>(codes8<E>(kw[2 * u], kw[2 * u + 1]), qf[u], s[t]);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) s[t][i] = __builtin_fmaf(s[t][i], ksc[t], (float)ve[t]);
+      for (int n = 0; n < 4; ++n) s[u][n] = __builtin_fmaf(s[u][n], ks, (float)ve[u]);
     }
-    const bool masked = k0 + kStep - 1 > lmin;
     bool nan_v = false;
-    if (masked) {
+    if (k0 + kStep - 1 > x.lmin) {
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
+      for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int key = k0 + 16 * t + 4 * g + i;
-          if (key > lim) s[t][i] = NEG_INF;
+        for (int n = 0; n < 4; ++n) {
+          const int key = k0 + 16 * u + 4 * g + n;
+          if (key > lim) s[u][n] = NEG_INF;
 #pragma unroll
-          for (int w = 0; w < (VB + 3) / 4; ++w) {
-            if (key >= kend) vw[t][i][w] = 0;       // what lies behind the last key may be anything
-            nan_v |= has_nan(vw[t][i][w]);
+          for (int w = 0; w < T::VW; ++w) {
+            if (key >= x.keys) t[u].v[n][w] = 0;       // what lies behind the last key may be anything
+            nan_v |= has_nan(t[u].v[n][w]);
           }
         }
     }
@@ -319,23 +381,23 @@ __global__ __launch_bounds__(64 * kWaves) void attend_kernel(PagedArgs a, int ro
       m = mn;
       l *= alpha;
 #pragma unroll
-      for (int x = 0; x < VB; ++x) acc[x] *= alpha;
+      for (int n = 0; n < VB; ++n) acc[n] *= alpha;
     }
     float p[2][4];
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
+    for (int u = 0; u < 2; ++u) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) p[t][i] = fast_exp2(s[t][i] - m);
-      l = __builtin_fmaf((p[t][0] + p[t][1]) + (p[t][2] + p[t][3]), exp2i(-ve[t]), l);
+      for (int n = 0; n < 4; ++n) p[u][n] = fast_exp2(s[u][n] - m);
+      l = __builtin_fmaf((p[u][0] + p[u][1]) + (p[u][2] + p[u][3]), exp2i(-ve[u]), l);
     }
-    // V^T operand of dims block x: slots j = 4 t + i are keys (t, i), the lane's dim c VB + x
-    auto v_operand = [&](int x) __attribute__((always_inline)) {
+    // V^T operand of dims block y: slots j = 4 u + n are keys (u, n), the lane's dim c VB + y
+    auto v_operand = [&](int y) __attribute__((always_inline)) {
       u32x4 r;
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
-        const uint32_t lo = cvt_f16(vw[w >> 1][2 * (w & 1)][x >> 2], (x & 2) != 0);
-        const uint32_t hi = cvt_f16(vw[w >> 1][2 * (w & 1) + 1][x >> 2], (x & 2) != 0);
-        r[w] = __builtin_amdgcn_perm(hi, lo, x & 1 ? 0x07060302u : 0x05040100u);
+        const uint32_t lo = cvt_f16(t[w >> 1].v[2 * (w & 1)][y >> 2], (y & 2) != 0);
+        const uint32_t hi = cvt_f16(t[w >> 1].v[2 * (w & 1) + 1][y >> 2], (y & 2) != 0);
+        r[w] = __builtin_amdgcn_perm(hi, lo, y & 1 ? 0x07060302u : 0x05040100u);
       }
       return r;
     };
@@ -349,23 +411,39 @@ __global__ __launch_bounds__(64 * kWaves) void attend_kernel(PagedArgs a, int ro
       for (int w = 0; w < 4; ++w)
         seen[w] = pack2<F16>(s[w >> 1][2 * (w & 1)] == NEG_INF ? 0.f : 1.f, s[w >> 1][2 * (w & 1) + 1] == NEG_INF ? 0.f : 1.f);
 #pragma unroll
-      for (int x = 0; x < VB; ++x) {
-        u32x4 v = v_operand(x), is;
+      for (int y = 0; y < VB; ++y) {
+        u32x4 v = v_operand(y), is;
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
           const bool lo = (v[w] & 0x7FFFu) > 0x7C00u, hi = (v[w] & 0x7FFF0000u) > 0x7C000000u;
           is[w] = (lo ? 0x3C00u : 0u) | (hi ? 0x3C000000u : 0u);
           v[w] = (lo ? 0u : v[w] & 0xFFFFu) | (hi ? 0u : v[w] & 0xFFFF0000u);
         }
-        acc[x] = mfma16<F16>(v, pf, acc[x]);
+        acc[y] = mfma16<F16>(v, pf, acc[y]);
         const f32x4 count = mfma16<F16>(is, seen, f32x4{});
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (count[i] > 0.f) acc[x][i] = __builtin_nanf("");
+        for (int n = 0; n < 4; ++n)
+          if (count[n] > 0.f) acc[y][n] = __builtin_nanf("");
       }
     } else {
 #pragma unroll
-      for (int x = 0; x < VB; ++x) acc[x] = mfma16<F16>(v_operand(x), pf, acc[x]);
+      for (int y = 0; y < VB; ++y) acc[y] = mfma16<F16>(v_operand(y), pf, acc[y]);
+    }
+  };
+
+  // The next step's bytes are on their way while a step is computed; past the last one its own
+  // are read once more, never past the run.
+  for (int j0 = 0; j0 < steps; j0 += 32) {
+    load_run(j0);
+    const int n = min(steps - j0, 32);
+    T ta[2], tb[2];
+    load_tile(ta[0], 0), load_tile(ta[1], 1);
+    for (int j = 0; j < n; j += 2) {
+      const int j1 = min(j + 1, n - 1), j2 = min(j + 2, n - 1);
+      load_tile(tb[0], 2 * j1), load_tile(tb[1], 2 * j1 + 1);
+      compute(ta, 2 * j, first + ((j0 + j) * kWaves + wave) * kStep);
+      load_tile(ta[0], 2 * j2), load_tile(ta[1], 2 * j2 + 1);
+      if (j + 1 < n) compute(tb, 2 * j + 2, first + ((j0 + j + 1) * kWaves + wave) * kStep);
     }
   }
 
@@ -374,14 +452,14 @@ __global__ __launch_bounds__(64 * kWaves) void attend_kernel(PagedArgs a, int ro
 #pragma unroll
   for (int i = 0; i < 4; ++i)
 #pragma unroll
-    for (int x = 0; x < VB; ++x) merge[wave][c][(4 * g + i) * VB + x] = acc[x][i];
+    for (int y = 0; y < VB; ++y) merge[wave][c][(4 * g + i) * VB + y] = acc[y][i];
   if (g == 0) ml[wave][0][c] = m, ml[wave][1][c] = l;
   __syncthreads();
   constexpr int PER = kRows * D / (64 * kWaves);   // values per thread (D = 32: 2)
   constexpr int TR = D / PER;                      // threads per row
   const int row = threadIdx.x / TR, d0 = threadIdx.x % TR * PER;
-  const int rr = r0 + row;
-  if (rr >= rows) return;
+  const int rr = x.r0 + row;
+  if (rr >= x.rows) return;
   const int ot = rr / G, oh = hk * G + rr % G;
   float M = -__FLT_MAX__, f[kWaves], L = 0.f, o[PER];
 #pragma unroll
@@ -393,18 +471,76 @@ __global__ __launch_bounds__(64 * kWaves) void attend_kernel(PagedArgs a, int ro
   }
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
-    float x = 0.f;
+    float z = 0.f;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) x = __builtin_fmaf(f[w], merge[w][row][d0 + i], x);
-    o[i] = x;
+    for (int w = 0; w < kWaves; ++w) z = __builtin_fmaf(f[w], merge[w][row][d0 + i], z);
+    o[i] = z;
   }
-  const bool live = ot < fresh;
+  if (per < x.keys) {   // more than one split: the join divides
+    float* const dst = part_row<D>(a, block, split, row);
+#pragma unroll
+    for (int i = 0; i < PER; ++i) dst[d0 + i] = o[i];
+    if (d0 == 0) dst[D] = M, dst[D + 1] = L;
+    return;
+  }
+  const bool live = ot < x.fresh;
   const float inv = live ? 1.0f / L : 0.f;
   uint16_t* dst = static_cast<uint16_t*>(const_cast<void*>(a.o.data)) + b * a.o.stride_b + oh * a.o.stride_h + ot * a.o.stride_n + d0;
 #pragma unroll
   for (int i = 0; i < PER; i += 2)
     *reinterpret_cast<uint32_t*>(dst + i) = live ? pack2<E>(o[i] * inv, o[i + 1] * inv) : 0u;
   if (a.lse != nullptr && d0 == 0) a.lse[((long long)b * a.H + oh) * a.N + ot] = live ? M + __log2f(L) : NEG_INF;
+}
+
+// Joins the splits of a row, a wave to a row; rows of blocks that were not split are there already.
+template <typename E, int D>
+__global__ __launch_bounds__(256) void join_kernel(PagedArgs a, int row_blocks) {
+  constexpr int PER = D >= 128 ? 2 : 1;
+  const int lane = threadIdx.x & 63;
+  const int Hkv = a.cache.H_kv, G = a.H / Hkv, rows = a.N * G;
+  const long long i = (long long)blockIdx.x * 4 + threadIdx.x / 64;   // (batch, K/V head), row
+  if (i >= (long long)a.B * Hkv * rows) return;
+  const int bh = i / rows, rr = i % rows, b = bh / Hkv, hk = bh % Hkv;
+  const Block x = block_of(a, b, rr / kRows, G);
+  const int per = split_keys(x.keys, a.nsplit);
+  if (per >= x.keys) return;
+  const int n = (x.keys + per - 1) / per;
+  const long long block = (long long)bh * row_blocks + rr / kRows;
+  float M = -__FLT_MAX__, L = 0.f, o[PER];
+#pragma unroll
+  for (int e = 0; e < PER; ++e) o[e] = 0.f;
+  for (int s0 = 0; s0 < n; s0 += 64) {
+    const int k = min(n - s0, 64);
+    const float* const mine = part_row<D>(a, block, s0 + min(lane, k - 1), rr % kRows);
+    const float ms = mine[D], ls = lane < k ? mine[D + 1] : 0.f;
+    float top = ms;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
+    const float Mn = fmaxf(M, top), back = fast_exp2(M - Mn), f = fast_exp2(ms - Mn);
+    M = Mn;
+    float sum = f * ls;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) sum += __shfl_xor(sum, d);
+    L = __builtin_fmaf(L, back, sum);
+#pragma unroll
+    for (int e = 0; e < PER; ++e) o[e] *= back;
+#pragma unroll 8
+    for (int s = 0; s < k; ++s) {
+      const float fs = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f), s));
+      const float* const p = part_row<D>(a, block, s0 + s, rr % kRows) + (lane * PER) % D;
+#pragma unroll
+      for (int e = 0; e < PER; ++e) o[e] = __builtin_fmaf(fs, p[e], o[e]);
+    }
+  }
+  const int ot = rr / G, oh = hk * G + rr % G;
+  const bool live = ot < x.fresh;
+  const float inv = live ? 1.0f / L : 0.f;
+  uint16_t* dst = static_cast<uint16_t*>(const_cast<void*>(a.o.data)) + b * a.o.stride_b + oh * a.o.stride_h + ot * a.o.stride_n;
+  if (lane * PER < D) {
+    if constexpr (PER == 2) *reinterpret_cast<uint32_t*>(dst + 2 * lane) = live ? pack2<E>(o[0] * inv, o[1] * inv) : 0u;
+    else dst[lane] = live ? (uint16_t)pack2<E>(o[0] * inv, 0.f) : 0;
+  }
+  if (a.lse != nullptr && lane == 0) a.lse[((long long)b * a.H + oh) * a.N + ot] = live ? M + __log2f(L) : -__builtin_inff();
 }
 
 // ---------------------------------------------------------------------------
@@ -442,12 +578,32 @@ int launch_append(AppendArgs a) {
                            : launch_append_passes<E, D, false>(a, (int)q_blocks, q_chunks, touched, items + q_blocks);
 }
 
+// Splits of each row block's keys: enough workgroups for every CU's share of kPerCu, none with fewer keys
+// than one step of its waves.
+constexpr int kPerCu = 4, kMaxSplit = 128;
+
+int split_of(int B, int Hkv, int row_blocks, long long keys) {
+  const long long blocks = (long long)B * Hkv * row_blocks;
+  const long long want = (kPerCu * (long long)cu_count() + blocks - 1) / blocks;
+  const long long most = (keys + kWaves * kStep - 1) / (kWaves * kStep);
+  return (int)std::max<long long>(1, std::min<long long>({want, most, kMaxSplit}));
+}
+
+int row_blocks_of(int N, int G) { return (int)(((long long)N * G + kRows - 1) / kRows); }
+
+size_t part_bytes(int B, int Hkv, int row_blocks, int nsplit, int D) {
+  return nsplit <= 1 ? 0 : (size_t)B * Hkv * row_blocks * nsplit * kRows * (D + 4) * sizeof(float);
+}
+
 template <typename E, int D>
 int launch_attend(const PagedArgs& a) {
-  const int rows = a.N * (a.H / a.cache.H_kv), row_blocks = (rows + kRows - 1) / kRows;
-  const long long grid = (long long)a.B * a.cache.H_kv * row_blocks;
-  if (grid > 0x7fffffffLL) return FA_ERR_DIMS;
+  const int row_blocks = row_blocks_of(a.N, a.H / a.cache.H_kv);
+  const long long grid = (long long)a.B * a.cache.H_kv * row_blocks * a.nsplit;
+  const long long joins = ((long long)a.B * a.H * a.N + 3) / 4;
+  if (grid > 0x7fffffffLL || joins > 0x7fffffffLL) return FA_ERR_DIMS;
   hipLaunchKernelGGL((attend_kernel<E, D>), dim3((unsigned)grid), dim3(64 * kWaves), 0, (hipStream_t)a.stream, a, row_blocks);
+  if (a.nsplit > 1)
+    hipLaunchKernelGGL((join_kernel<E, D>), dim3((unsigned)joins), dim3(256), 0, (hipStream_t)a.stream, a, row_blocks);
   return hipGetLastError() == hipSuccess ? FA_OK : FA_ERR_LAUNCH;
 }
 
@@ -464,7 +620,10 @@ int paged_append(int dtype, const AppendArgs& a) {
   return launch_append<F16, 128>(a);
 }
 
-int paged_attention(int dtype, PagedArgs a, size_t) {
+int paged_attention(int dtype, PagedArgs a, size_t workspace_bytes) {
+  const int Hkv = a.cache.H_kv, row_blocks = row_blocks_of(a.N, a.H / Hkv);
+  a.nsplit = split_of(a.B, Hkv, row_blocks, (long long)a.cache.table_width * a.cache.page_size);
+  while (a.nsplit > 1 && part_bytes(a.B, Hkv, row_blocks, a.nsplit, a.D) > workspace_bytes) --a.nsplit;
   if (dtype == FA_BF16) {
     if (a.D == 32) return launch_attend<BF16, 32>(a);
     if (a.D == 64) return launch_attend<BF16, 64>(a);
@@ -475,6 +634,9 @@ int paged_attention(int dtype, PagedArgs a, size_t) {
   return launch_attend<F16, 128>(a);
 }
 
-size_t paged_attention_workspace(int, int, int, int, int, long long) { return 0; }
+size_t paged_attention_workspace(int B, int H, int Hkv, int N, int D, long long keys) {
+  const int row_blocks = row_blocks_of(N, H / Hkv);
+  return part_bytes(B, Hkv, row_blocks, split_of(B, Hkv, row_blocks, keys), D);
+}
 
 }  // namespace fa
