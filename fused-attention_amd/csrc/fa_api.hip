@@ -91,6 +91,7 @@ int check_rows(const fa_rows& r) {
 
 int check_rotation(const fa_rotation& r, int D, int dtype) {
   if ((r.q_weight || r.k_weight) && r.weight_dtype != dtype && r.weight_dtype != FA_F32) return FA_ERR_ROTATION;
+  if (!aligned16(r.q_weight) || !aligned16(r.k_weight)) return FA_ERR_ROTATION;
   if (!r.table) return FA_OK;
   if (!aligned16(r.table) || r.table_len <= 0) return FA_ERR_ROTATION;
   if (r.rotary_dim <= 0 || r.rotary_dim > D || r.rotary_dim % 16 != 0) return FA_ERR_ROTATION;

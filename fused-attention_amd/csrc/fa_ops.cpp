@@ -158,12 +158,12 @@ Rotation rotation_of(const Tensor& x, const OptTensor& wq, const OptTensor& wk, 
 void place(Rotation& t, const Tensor& x) {
   if (t.wq.defined()) {
     check_device(t.wq, x, "q_weight");
-    t.wq = t.wq.contiguous();
+    t.wq = dense16(t.wq);
     t.r.q_weight = t.wq.data_ptr();
   }
   if (t.wk.defined()) {
     check_device(t.wk, x, "k_weight");
-    t.wk = t.wk.contiguous();
+    t.wk = dense16(t.wk);
     t.r.k_weight = t.wk.data_ptr();
   }
   const Tensor& w = t.wq.defined() ? t.wq : t.wk;

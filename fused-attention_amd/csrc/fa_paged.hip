@@ -106,10 +106,10 @@ __global__ __launch_bounds__(kRowThreads) void append_kernel(AppendArgs a, int q
   const Rows& in = is_k ? a.k : a.v;
   const uint16_t* src = static_cast<const uint16_t*>(in.data) + b * in.stride_b + h * in.stride_h + d0;
 
-  float y[PASSES][8];
+  float y[PASSES][8], own[8], other[8];
   float amax = 0.f;
-#pragma unroll
-  for (int p = 0; p < PASSES; ++p) {
+  if (is_k) load_weights<INTER>(a.rot, a.rot.k_weight, d0, own, other);
+  auto pass = [&](int p, float (&z)[8]) __attribute__((always_inline)) {
     const int n = first + p * S::TOKENS + slot - past;
     const bool live = p * S::TOKENS + slot < ps && n >= 0 && n < fresh;
     const int nn = live ? n : 0;
@@ -118,15 +118,26 @@ __global__ __launch_bounds__(kRowThreads) void append_kernel(AppendArgs a, int q
       Turn<D, INTER> turn;
       turn.load(a.rot, lane, d0, b, nn, (long long)past + nn);
       float cw[8], sw[8];
-      fold_weight<INTER>(turn.c, turn.s, a.rot, a.rot.k_weight, d0, cw, sw);
-      turn_row<E, D, INTER>(w, turn.fetch(w), cw, sw, a.rot.k_weight != nullptr, a.rot.eps, y[p]);
+      fold_weights(turn, own, other, cw, sw);
+      turn_row<E, D, INTER>(w, turn.fetch(w), cw, sw, a.rot.k_weight != nullptr, a.rot.eps, z);
     } else {
-      unpack8<E>(w, y[p]);
+      unpack8<E>(w, z);
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float x = __builtin_fabsf(y[p][i]);
+      const float x = __builtin_fabsf(z[i]);
       if (live && x < __builtin_inff()) amax = fmaxf(amax, x);
+    }
+  };
+  // (a page of which a few rows are new skips the passes without one; all new, no branch parts their loads)
+  if (held == 0 && first + ps <= past + fresh) {
+#pragma unroll
+    for (int p = 0; p < PASSES; ++p) pass(p, y[p]);
+  } else {
+#pragma unroll
+    for (int p = 0; p < PASSES; ++p) {
+      const int n = first + p * S::TOKENS - past;
+      if (n + S::TOKENS > 0 && n < fresh) pass(p, y[p]);
     }
   }
 #pragma unroll
@@ -178,6 +189,7 @@ __global__ __launch_bounds__(kRowThreads) void append_kernel(AppendArgs a, int q
 constexpr int kWaves = 4;
 constexpr int kRows = 16;
 constexpr int kStep = 32;   // keys per step of a wave
+constexpr int kMaxSplit = 128;
 constexpr float kLazy = 15.f, kBelow = 7.f;
 
 __device__ __forceinline__ uint32_t cvt_f16(uint32_t w, bool hi) {
@@ -492,55 +504,68 @@ __global__ __launch_bounds__(64 * kWaves) void attend_kernel(PagedArgs a, int ro
   if (a.lse != nullptr && d0 == 0) a.lse[((long long)b * a.H + oh) * a.N + ot] = live ? M + __log2f(L) : NEG_INF;
 }
 
-// Joins the splits of a row, a wave to a row; rows of blocks that were not split are there already.
+// Joins the splits of a row, a workgroup to a row: D / 4 threads a split, 1024 / D splits at a time.
+// Rows of blocks that were not split are there already.
+constexpr int kJoinThreads = 256;
+
 template <typename E, int D>
-__global__ __launch_bounds__(256) void join_kernel(PagedArgs a, int row_blocks) {
-  constexpr int PER = D >= 128 ? 2 : 1;
-  const int lane = threadIdx.x & 63;
+__global__ __launch_bounds__(kJoinThreads) void join_kernel(PagedArgs a, int row_blocks) {
+  constexpr int TR = D / 4, PAR = kJoinThreads / TR;
+  __shared__ float ml[kMaxSplit][2];
+  __shared__ __attribute__((aligned(16))) float sums[PAR][D];
   const int Hkv = a.cache.H_kv, G = a.H / Hkv, rows = a.N * G;
-  const long long i = (long long)blockIdx.x * 4 + threadIdx.x / 64;   // (batch, K/V head), row
-  if (i >= (long long)a.B * Hkv * rows) return;
-  const int bh = i / rows, rr = i % rows, b = bh / Hkv, hk = bh % Hkv;
+  const int bh = blockIdx.x / rows, rr = blockIdx.x % rows, b = bh / Hkv, hk = bh % Hkv;
   const Block x = block_of(a, b, rr / kRows, G);
   const int per = split_keys(x.keys, a.nsplit);
   if (per >= x.keys) return;
   const int n = (x.keys + per - 1) / per;
   const long long block = (long long)bh * row_blocks + rr / kRows;
-  float M = -__FLT_MAX__, L = 0.f, o[PER];
+  const int p = threadIdx.x / TR, d0 = threadIdx.x % TR * 4;
+  const float* const src = part_row<D>(a, block, 0, rr % kRows);
+  constexpr int STRIDE = kRows * (D + 4);
+  if (threadIdx.x < n) {
+    ml[threadIdx.x][0] = src[threadIdx.x * STRIDE + D];
+    ml[threadIdx.x][1] = src[threadIdx.x * STRIDE + D + 1];
+  }
+  // (the sums' loads do not wait for the factors)
+  constexpr int AHEAD = kMaxSplit / PAR < 8 ? kMaxSplit / PAR : 8;
+  f32x4 v[AHEAD];
 #pragma unroll
-  for (int e = 0; e < PER; ++e) o[e] = 0.f;
-  for (int s0 = 0; s0 < n; s0 += 64) {
-    const int k = min(n - s0, 64);
-    const float* const mine = part_row<D>(a, block, s0 + min(lane, k - 1), rr % kRows);
-    const float ms = mine[D], ls = lane < k ? mine[D + 1] : 0.f;
-    float top = ms;
+  for (int i = 0; i < AHEAD; ++i) v[i] = gload_f32x4(src + min(p + i * PAR, n - 1) * STRIDE + d0);
+  __syncthreads();
+  float M = -__FLT_MAX__, L = 0.f;
+  for (int s = 0; s < n; ++s) M = fmaxf(M, ml[s][0]);
+  for (int s = 0; s < n; ++s) L = __builtin_fmaf(fast_exp2(ml[s][0] - M), ml[s][1], L);
+  f32x4 o = f32x4{};
 #pragma unroll
-    for (int d = 1; d < 64; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
-    const float Mn = fmaxf(M, top), back = fast_exp2(M - Mn), f = fast_exp2(ms - Mn);
-    M = Mn;
-    float sum = f * ls;
+  for (int i = 0; i < AHEAD; ++i) {
+    const int s = p + i * PAR;
+    const float f = s < n ? fast_exp2(ml[s][0] - M) : 0.f;
 #pragma unroll
-    for (int d = 1; d < 64; d *= 2) sum += __shfl_xor(sum, d);
-    L = __builtin_fmaf(L, back, sum);
+    for (int e = 0; e < 4; ++e) o[e] = s < n ? __builtin_fmaf(f, v[i][e], o[e]) : o[e];
+  }
+  for (int s = p + AHEAD * PAR; s < n; s += PAR) {
+    const float f = fast_exp2(ml[s][0] - M);
+    const f32x4 w = gload_f32x4(src + s * STRIDE + d0);
 #pragma unroll
-    for (int e = 0; e < PER; ++e) o[e] *= back;
-#pragma unroll 8
-    for (int s = 0; s < k; ++s) {
-      const float fs = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f), s));
-      const float* const p = part_row<D>(a, block, s0 + s, rr % kRows) + (lane * PER) % D;
+    for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(f, w[e], o[e]);
+  }
+  *reinterpret_cast<f32x4*>(&sums[p][d0]) = o;
+  __syncthreads();
+  if (threadIdx.x >= D / 2) return;
+  float z[2] = {0.f, 0.f};
 #pragma unroll
-      for (int e = 0; e < PER; ++e) o[e] = __builtin_fmaf(fs, p[e], o[e]);
-    }
+  for (int i = 0; i < PAR; ++i) {
+    z[0] += sums[i][2 * threadIdx.x];
+    z[1] += sums[i][2 * threadIdx.x + 1];
   }
   const int ot = rr / G, oh = hk * G + rr % G;
   const bool live = ot < x.fresh;
   const float inv = live ? 1.0f / L : 0.f;
   uint16_t* dst = static_cast<uint16_t*>(const_cast<void*>(a.o.data)) + b * a.o.stride_b + oh * a.o.stride_h + ot * a.o.stride_n;
-  if (lane * PER < D) {
-    if constexpr (PER == 2) *reinterpret_cast<uint32_t*>(dst + 2 * lane) = live ? pack2<E>(o[0] * inv, o[1] * inv) : 0u;
-    else dst[lane] = live ? (uint16_t)pack2<E>(o[0] * inv, 0.f) : 0;
-  }
-  if (a.lse != nullptr && lane == 0) a.lse[((long long)b * a.H + oh) * a.N + ot] = live ? M + __log2f(L) : -__builtin_inff();
+  *reinterpret_cast<uint32_t*>(dst + 2 * threadIdx.x) = live ? pack2<E>(z[0] * inv, z[1] * inv) : 0u;
+  if (a.lse != nullptr && threadIdx.x == 0)
+    a.lse[((long long)b * a.H + oh) * a.N + ot] = live ? M + __log2f(L) : -__builtin_inff();
 }
 
 // ---------------------------------------------------------------------------
@@ -580,7 +605,7 @@ int launch_append(AppendArgs a) {
 
 // Splits of each row block's keys: enough workgroups for every CU's share of kPerCu, none with fewer keys
 // than one step of its waves.
-constexpr int kPerCu = 4, kMaxSplit = 128;
+constexpr int kPerCu = 4;
 
 int split_of(int B, int Hkv, int row_blocks, long long keys) {
   const long long blocks = (long long)B * Hkv * row_blocks;
@@ -599,11 +624,11 @@ template <typename E, int D>
 int launch_attend(const PagedArgs& a) {
   const int row_blocks = row_blocks_of(a.N, a.H / a.cache.H_kv);
   const long long grid = (long long)a.B * a.cache.H_kv * row_blocks * a.nsplit;
-  const long long joins = ((long long)a.B * a.H * a.N + 3) / 4;
+  const long long joins = (long long)a.B * a.H * a.N;
   if (grid > 0x7fffffffLL || joins > 0x7fffffffLL) return FA_ERR_DIMS;
   hipLaunchKernelGGL((attend_kernel<E, D>), dim3((unsigned)grid), dim3(64 * kWaves), 0, (hipStream_t)a.stream, a, row_blocks);
   if (a.nsplit > 1)
-    hipLaunchKernelGGL((join_kernel<E, D>), dim3((unsigned)joins), dim3(256), 0, (hipStream_t)a.stream, a, row_blocks);
+    hipLaunchKernelGGL((join_kernel<E, D>), dim3((unsigned)joins), dim3(kJoinThreads), 0, (hipStream_t)a.stream, a, row_blocks);
   return hipGetLastError() == hipSuccess ? FA_OK : FA_ERR_LAUNCH;
 }
 

@@ -55,13 +55,9 @@ struct Turn {
     return d0 < half ? lane + half / 8 : lane - half / 8;
   }
 
-  // Position of a pair: its axis by the sections, the token's entry of that axis.  `base`: the
-  // position when no positions are given.
-  __device__ __forceinline__ static long long position(const RotaryArgs& a, int pair, int b, int n, long long base) {
+  // The token's entry of an axis; `base`: its position when none are given.
+  __device__ __forceinline__ static long long position(const RotaryArgs& a, int axis, int b, int n, long long base) {
     if (a.positions == nullptr) return base;
-    int axis = 0;
-#pragma unroll
-    for (int i = 0; i < kMaxAxes - 1; ++i) axis += i < a.axes - 1 && pair >= a.section_end[i] ? 1 : 0;
     const long long at = axis * a.pos_axis_stride + (long long)b * a.pos_batch_stride + n;
     return a.positions_int64 ? static_cast<const long long*>(a.positions)[at] : static_cast<const int*>(a.positions)[at];
   }
@@ -96,14 +92,23 @@ struct Turn {
         ss[i] = p < 0 ? 0.f : ss[i] + bad;
       }
     } else {
+      // (every axis' position, then every table value: two waits, not two a pair)
+      const long long p0 = position(a, 0, b, n, base), p1 = position(a, 1, b, n, base);
+      const long long p2 = a.axes > 2 ? position(a, 2, b, n, base) : p1;
+      const int end0 = a.section_end[0], end1 = a.axes > 2 ? a.section_end[1] : half;
+      long long p[NP];
+#pragma unroll
+      for (int i = 0; i < NP; ++i) p[i] = pair0 + i < end0 ? p0 : pair0 + i < end1 ? p1 : p2;
 #pragma unroll
       for (int i = 0; i < NP; ++i) {
-        const long long p = position(a, pair0 + i, b, n, base);
-        const bool in = p >= 0 && p < a.table_len;
-        const float* row = a.table + (in ? p : 0) * a.rotary_dim + pair0 + i;
-        const float x = row[0], y = row[half];
-        cc[i] = in ? x : p < 0 ? 1.f : __builtin_nanf("");
-        ss[i] = in ? y : p < 0 ? 0.f : __builtin_nanf("");
+        const float* row = a.table + (p[i] >= 0 && p[i] < a.table_len ? p[i] : 0) * a.rotary_dim + pair0 + i;
+        cc[i] = row[0], ss[i] = row[half];
+      }
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+        const float bad = p[i] >= a.table_len ? __builtin_nanf("") : 0.f;
+        cc[i] = p[i] < 0 ? 1.f : cc[i] + bad;
+        ss[i] = p[i] < 0 ? 0.f : ss[i] + bad;
       }
     }
     if constexpr (INTER) {
@@ -136,14 +141,20 @@ __device__ __forceinline__ float partner_of(const float (&xp)[8], int i) {
   return INTER ? xp[i ^ 1] : xp[i];
 }
 
-// Norm weight of dims d0 .. d0 + 7 (ones without one).
+// Norm weight of dims d0 .. d0 + 7 (ones without one), 16-byte aligned.
 __device__ __forceinline__ void load_weight(const RotaryArgs& a, const void* w, int d0, float (&x)[8]) {
+  if (w == nullptr) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    if (w == nullptr) x[i] = 1.f;
-    else if (a.weight_dtype == FA_F32) x[i] = static_cast<const float*>(w)[d0 + i];
-    else if (a.weight_dtype == FA_BF16) x[i] = to_f32<BF16>(static_cast<const uint16_t*>(w)[d0 + i]);
-    else x[i] = to_f32<F16>(static_cast<const uint16_t*>(w)[d0 + i]);
+    for (int i = 0; i < 8; ++i) x[i] = 1.f;
+  } else if (a.weight_dtype == FA_F32) {
+    const float* const p = static_cast<const float*>(w) + d0;
+    const f32x4 lo = gload_f32x4(p), hi = gload_f32x4(p + 4);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = lo[i], x[4 + i] = hi[i];
+  } else {
+    const u32x4 v = gload16(static_cast<const uint16_t*>(w) + d0);
+    if (a.weight_dtype == FA_BF16) unpack8<BF16>(v, x);
+    else unpack8<F16>(v, x);
   }
 }
 
@@ -167,18 +178,23 @@ __device__ __forceinline__ void turn_row(const u32x4& w, const u32x4& wp, const 
   for (int i = 0; i < 8; ++i) y[i] = r * __builtin_fmaf(x[i], cw[i], partner_of<INTER>(xp, i) * sw[i]);
 }
 
+// The weights of a lane's dims and of their partners (in place of the partners' own order when
+// interleaved: partner_of picks them).
 template <bool INTER>
-__device__ __forceinline__ void fold_weight(const float (&c)[8], const float (&s)[8], const RotaryArgs& a, const void* w,
-                                            int d0, float (&cw)[8], float (&sw)[8]) {
-  float own[8], other[8];
-  load_weight(a, w, d0, own);
+__device__ __forceinline__ void load_weights(const RotaryArgs& a, const void* w, int d0, float (&own)[8], float (&other)[8]) {
   const int half = a.rotary_dim / 2;
   const bool turned = a.table != nullptr && d0 < a.rotary_dim;
+  load_weight(a, w, d0, own);
   load_weight(a, w, INTER || !turned ? d0 : d0 < half ? d0 + half : d0 - half, other);
+}
+
+template <int D, bool INTER>
+__device__ __forceinline__ void fold_weights(const Turn<D, INTER>& t, const float (&own)[8], const float (&other)[8],
+                                             float (&cw)[8], float (&sw)[8]) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    cw[i] = c[i] * own[i];
-    sw[i] = s[i] * partner_of<INTER>(other, i);
+    cw[i] = t.c[i] * own[i];
+    sw[i] = t.s[i] * partner_of<INTER>(other, i);
   }
 }
 
@@ -197,10 +213,11 @@ template <typename E, int D, bool INTER>
 __device__ __forceinline__ void turn_heads(const RotaryArgs& rot, const void* w, const Rows& in, const Rows& out, int b,
                                            int n, long long base, int h0, int h1, bool valid) {
   const int d0 = (threadIdx.x % Slot<D>::TPR) * 8;
+  float own[8], other[8], cw[8], sw[8];
+  load_weights<INTER>(rot, w, d0, own, other);
   Turn<D, INTER> turn;
   turn.load(rot, threadIdx.x & 63, d0, b, n, base);
-  float cw[8], sw[8];
-  fold_weight<INTER>(turn.c, turn.s, rot, w, d0, cw, sw);
+  fold_weights(turn, own, other, cw, sw);
   const uint16_t* src = static_cast<const uint16_t*>(in.data) + b * in.stride_b + n * in.stride_n + d0;
   uint16_t* dst = static_cast<uint16_t*>(const_cast<void*>(out.data)) + b * out.stride_b + n * out.stride_n + d0;
   for (int h = h0; h < h1; h += kRowBatch) {

@@ -111,27 +111,30 @@ __global__ __launch_bounds__(kRowThreads) void qk_bwd_kernel(QkArgs a, int q_chu
   }
 }
 
-// dw of q (blockIdx.y 0) or k (1): the rows of `part` of their chunks, 16 columns to a workgroup.
+// dw of q (blockIdx.y 0) or k (1): the rows of `part` of their chunks, 4 columns to a workgroup.
 template <typename E, int D>
 __global__ __launch_bounds__(kRowThreads) void qk_dw_kernel(QkArgs a, int q_chunks, int chunks) {
   const bool is_q = blockIdx.y == 0;
-  const int col = blockIdx.x * 16 + threadIdx.x % 16, r = threadIdx.x / 16;
+  const int c = blockIdx.x * 4;
   const long long first = is_q ? 0 : (long long)q_chunks * a.blocks;
   const long long rows = (long long)(is_q ? q_chunks : chunks - q_chunks) * a.blocks;
-  float x = 0.f;
-#pragma unroll 8
-  for (long long i = r; i < rows; i += 16) x += a.part[(first + i) * D + col];
-  __shared__ float sums[16][17];
-  sums[r][threadIdx.x % 16] = x;
+  f32x4 x = f32x4{};
+#pragma unroll 4
+  for (long long i = threadIdx.x; i < rows; i += kRowThreads) x += gload_f32x4(a.part + (first + i) * D + c);
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] += __shfl_xor(x[i], d);
+  __shared__ f32x4 sums[kRowThreads / 64];
+  if (threadIdx.x % 64 == 0) sums[threadIdx.x / 64] = x;
   __syncthreads();
-  if (threadIdx.x < 16) {
+  if (threadIdx.x < 4) {
     float s = 0.f;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) s += sums[i][threadIdx.x];
+    for (int i = 0; i < kRowThreads / 64; ++i) s += sums[i][threadIdx.x];
     void* const dst = is_q ? a.dwq : a.dwk;
-    const int c = blockIdx.x * 16 + threadIdx.x;
-    if (a.rot.weight_dtype == FA_F32) static_cast<float*>(dst)[c] = s;
-    else static_cast<uint16_t*>(dst)[c] = (uint16_t)pack2<E>(s, s);
+    if (a.rot.weight_dtype == FA_F32) static_cast<float*>(dst)[c + threadIdx.x] = s;
+    else static_cast<uint16_t*>(dst)[c + threadIdx.x] = (uint16_t)pack2<E>(s, s);
   }
 }
 
@@ -171,7 +174,7 @@ int launch_qk(QkArgs a, bool bwd) {
     if (a.rot.interleaved) hipLaunchKernelGGL((qk_bwd_kernel<E, D, true>), g, t, 0, st, a, p.q_chunks, p.chunks);
     else hipLaunchKernelGGL((qk_bwd_kernel<E, D, false>), g, t, 0, st, a, p.q_chunks, p.chunks);
     if (a.rot.q_weight != nullptr)
-      hipLaunchKernelGGL((qk_dw_kernel<E, D>), dim3(D / 16, 2), t, 0, st, a, p.q_chunks, p.chunks);
+      hipLaunchKernelGGL((qk_dw_kernel<E, D>), dim3(D / 4, 2), t, 0, st, a, p.q_chunks, p.chunks);
   } else {
     if (a.rot.interleaved) hipLaunchKernelGGL((qk_fwd_kernel<E, D, true>), g, t, 0, st, a, p.q_chunks, p.chunks);
     else hipLaunchKernelGGL((qk_fwd_kernel<E, D, false>), g, t, 0, st, a, p.q_chunks, p.chunks);

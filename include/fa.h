@@ -216,7 +216,8 @@ FA_API size_t fa_bwd_gqa_workspace_size(int B, int H, int H_kv, int S, int D);
  * Rows are [B, heads, N, D], D contiguous, the other strides free (in elements, multiples of 8; data
  * 16-byte aligned), so the views of a packed projection [B, N, heads, D] are read as they are.
  * fa_rotation:
- *   q_weight, k_weight : norm weights [D] of weight_dtype (the rows' type or FA_F32); NULL, both: no norm
+ *   q_weight, k_weight : norm weights [D] of weight_dtype (the rows' type or FA_F32), 16-byte
+ *            aligned; NULL, both: no norm
  *   table  : [table_len, rotary_dim] fp32, the cosines of the rotary_dim / 2 pairs, then their sines;
  *            16-byte aligned; NULL: no rotation.  rotary_dim: a multiple of 16 up to D; dims past it keep
  *            their normed value.  Pair j is dims (j, j + rotary_dim / 2), or (2j, 2j + 1) if interleaved.

@@ -155,6 +155,8 @@ def test_strides_alignment_and_broadcast():
     wide = torch.randn(3, 20, 4, D + 4, generator=gen(7), device="cuda").to(dt)[..., :D].transpose(1, 2)  # row stride 68
     every = torch.randn(3, 4, 20, 2 * D, generator=gen(8), device="cuda").to(dt)[..., ::2]      # dims not contiguous
     check(wide, every, wq, wk, table, None, None, True, label="wide")
+    off = torch.empty(D + 8, device="cuda", dtype=dt)[1:1 + D].copy_(wq)
+    check(odd, k, off, wk, table[:, ::1], None, None, False, label="weight off 16 bytes")
     # the gradient of a broadcast input is the sum over what it was broadcast to
     one = k[:, :1].detach().clone().requires_grad_(True)
     q = odd.detach()

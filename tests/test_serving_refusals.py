@@ -188,6 +188,7 @@ def qk(lib, rows=None, rot=None, B=1, H=4, Hkv=2, N=8, D=64, dtype=0, bwd=False,
      _lib.FA_ERR_ROTATION),
     (dict(rot=Rotation(q_weight=FAKE)), _lib.FA_ERR_ROTATION),
     (dict(rot=Rotation(q_weight=FAKE, k_weight=FAKE, weight_dtype=1)), _lib.FA_ERR_ROTATION),
+    (dict(rot=Rotation(q_weight=FAKE, k_weight=FAKE + 4, weight_dtype=0)), _lib.FA_ERR_ROTATION),
 ])
 def test_rotary_entries_reject(lib, kw, code, bwd):
     assert qk(lib, bwd=bwd, **kw) == code
