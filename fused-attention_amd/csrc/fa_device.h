@@ -217,6 +217,17 @@ __device__ __forceinline__ void lds_write8(unsigned char* base, int byte_off, co
   *reinterpret_cast<u32x2*>(base + byte_off) = v;
 }
 
+typedef short i16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
+
+// Two 8-byte transposed LDS reads -> one 16-byte MFMA operand.
+__device__ __forceinline__ u32x4 lds_read_tr16x2(const unsigned char* base, int off0, int off1) {
+  i16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(base + off0));
+  i16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(base + off1));
+  u32x2 ua = __builtin_bit_cast(u32x2, a), ub = __builtin_bit_cast(u32x2, b);
+  return u32x4{ua[0], ua[1], ub[0], ub[1]};
+}
+
 // Buffer descriptor for raw byte-addressed loads from [p, p + bytes): word 3 =
 // 0x00020000 is the gfx9 setting for untyped dword access; loads past `bytes`
 // (vector offset) read zero.

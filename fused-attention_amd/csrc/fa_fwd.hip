@@ -66,9 +66,6 @@
 
 namespace fa {
 
-typedef short i16x4 __attribute__((ext_vector_type(4)));
-typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
-
 // s_waitcnt vmcnt(0) (expcnt and lgkmcnt left at their maxima)
 constexpr int kWaitVmcnt0 = 0x0F70;
 // p is recomputed against a fresh row max only when a row's sum of p over a
@@ -89,14 +86,6 @@ template <bool B>
 struct Tag {
   static constexpr bool value = B;
 };
-
-// Two 8-byte transposed LDS reads -> one 16-byte MFMA operand.
-__device__ __forceinline__ u32x4 lds_read_tr16x2(const unsigned char* base, int off0, int off1) {
-  i16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(base + off0));
-  i16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(base + off1));
-  u32x2 ua = __builtin_bit_cast(u32x2, a), ub = __builtin_bit_cast(u32x2, b);
-  return u32x4{ua[0], ua[1], ub[0], ub[1]};
-}
 
 // KS > 1: the keys of every tile are split over KS groups of WR waves (GH = 1).
 template <typename E, int D, int BM, int BN, int GH, int KS, bool LSE>

@@ -1,10 +1,6 @@
 // fa_paged.hip - keys and values in pages of 8-bit values with a scale for each page and head:
 // the append (norm, rotation, quantisation) and the attention over the pages, for gfx950.
-//
-// A value of a page is code 2^e, code an e4m3 number and 2^e the scale of its page and K/V head.
-// e4m3 is a floating format, so a scale only has to bring the page's largest value into range; with
-// powers of two it costs no rounding of its own, growing one moves the codes exactly (but for
-// subnormals), and both products below take it in exponent arithmetic.
+#include "fa_paged.h"
 #include "fa_rotary.h"
 
 #include <algorithm>
@@ -12,11 +8,6 @@
 namespace fa {
 
 typedef float f32x2 __attribute__((ext_vector_type(2)));
-
-constexpr int kScaleMin = -40, kScaleMax = 40;   // see attend: l needs the spread to stay far inside fp32's
-constexpr float kCodeMax = 448.f;
-
-__device__ __forceinline__ float exp2i(int e) { return __int_as_float((e + 127) << 23); }
 
 // The least e with amax <= 448 2^e (448 = 1.75 2^8), kept within the scales' range.
 __device__ __forceinline__ int scale_exponent(float amax) {
@@ -51,17 +42,6 @@ __device__ __forceinline__ void decode8(const u32x2& w, float (&y)[8]) {
     y[4 * i] = a[0], y[4 * i + 1] = a[1], y[4 * i + 2] = b[0], y[4 * i + 3] = b[1];
   }
 }
-
-// The page that the table names for column `col` of sequence b; -1: none.
-__device__ __forceinline__ int page_of(const fa_paged_cache& c, int b, int col) {
-  if (col >= c.table_width) return -1;
-  const int p = c.block_table[b * c.table_stride + col];
-  return p >= 0 && p < c.num_pages ? p : -1;
-}
-
-// Lengths as the kernels use them: nothing negative, no sum past 31 bits.
-__device__ __forceinline__ int past_of(const int* past, int b) { return min(max(past[b], 0), 0x3FFFFFFF); }
-__device__ __forceinline__ int fresh_of(const int* fresh, int b, int N) { return fresh ? min(max(fresh[b], 0), N) : N; }
 
 // ---------------------------------------------------------------------------
 // Append.  The first q_blocks workgroups turn the queries (turn_heads); each of the others owns one
@@ -101,8 +81,8 @@ __global__ __launch_bounds__(kRowThreads) void append_kernel(AppendArgs a, int q
   const int d0 = (threadIdx.x % S::TPR) * 8;
   const long long ph = (long long)page * Hkv + h;
   uint8_t* const codes = static_cast<uint8_t*>(is_k ? a.cache.k : a.cache.v) + ph * ps * D + d0;
-  uint8_t* const scale = static_cast<uint8_t*>(is_k ? a.cache.k_scale : a.cache.v_scale) + ph;
-  const int e_held = (int)*scale - 127;
+  void* const scales = is_k ? a.cache.k_scale : a.cache.v_scale;
+  const int e_held = scale_of(scales, ph);
   const Rows& in = is_k ? a.k : a.v;
   const uint16_t* src = static_cast<const uint16_t*>(in.data) + b * in.stride_b + h * in.stride_h + d0;
 
@@ -156,29 +136,18 @@ __global__ __launch_bounds__(kRowThreads) void append_kernel(AppendArgs a, int q
     if (row < ps && n >= 0 && n < fresh) *reinterpret_cast<u32x2*>(codes + row * D) = encode8(y[p], mul);
   }
   if (held > 0 && e > e_held) {
-    const float move = __builtin_ldexpf(1.f, max(e_held - e, -100));
+    const float move = exp2i(e_held - e);
     for (int row = slot; row < held; row += S::TOKENS) {
       float z[8];
       decode8(*reinterpret_cast<const u32x2*>(codes + row * D), z);
       *reinterpret_cast<u32x2*>(codes + row * D) = encode8(z, move);
     }
   }
-  if (threadIdx.x == 0) *scale = (uint8_t)(e + 127);
+  if (threadIdx.x == 0) static_cast<uint8_t*>(scales)[ph] = (uint8_t)(e + 127);
 }
 
 // ---------------------------------------------------------------------------
-// Attention over the pages.
-//
-//   s'_ij = (q_i . code_j) c 2^ke(page) + ve(page),  c = log2(e) / sqrt(D)
-//   p'_ij = 2^(s'_ij - m'),  acc_i = sum_j p'_ij vcode_j,  l_i = sum_j 2^-ve p'_ij,  o = acc / l
-//
-// The V scale sits in the exponent: p' is measured by what its key adds to the output, so its
-// rounding to 16 bits (fp16: 2^-11 relative, next to the largest contribution) is safe for any mix of
-// scales, one accumulator serves all pages, and l, in fp32, takes the scales out again.  (|ve| <= 40 keeps
-// 2^-ve p' of every key that counts inside fp32's normal range.)  The codes go into the products
-// unscaled, exact in both 16-bit types: QK in the queries' type, PV in fp16.  m' is lazy and low: it
-// moves, to 7 below the largest score, when a score passes it by more than 15.  So p' <= 2^15, and
-// the many small weights of a long flat tail stay above fp16's subnormals down to 2^-21 of the largest.
+// Attention of few rows (the mathematics: fa_paged.h).
 //
 // Rows: the N x G queries of a K/V head (G = H / H_kv), row r = token r / G, head r % G: 16 to a
 // workgroup, so each key's bytes serve all of them.  S^T = K Q^T as 16x16x32 products (16 keys x 16
@@ -189,28 +158,7 @@ __global__ __launch_bounds__(kRowThreads) void append_kernel(AppendArgs a, int q
 constexpr int kWaves = 4;
 constexpr int kRows = 16;
 constexpr int kStep = 32;   // keys per step of a wave
-constexpr int kMaxSplit = 128;
-constexpr float kLazy = 15.f, kBelow = 7.f;
-
-__device__ __forceinline__ uint32_t cvt_f16(uint32_t w, bool hi) {
-  const f16x2 r = hi ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.f, true) : __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.f, false);
-  return __builtin_bit_cast(uint32_t, r);
-}
-
-template <typename E>
-__device__ __forceinline__ u32x4 codes8(uint32_t w0, uint32_t w1) {
-  if constexpr (std::is_same<E, F16>::value) {
-    return u32x4{cvt_f16(w0, false), cvt_f16(w0, true), cvt_f16(w1, false), cvt_f16(w1, true)};
-  } else {
-    return u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w0, 1.f, false)),
-                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w0, 1.f, true)),
-                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w1, 1.f, false)),
-                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w1, 1.f, true))};
-  }
-}
-
-// Any byte of w a NaN code (0x7F, 0xFF)?
-__device__ __forceinline__ bool has_nan(uint32_t w) { return (((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u) != 0; }
+constexpr int kSplitStep = kWaves * kStep;
 
 // Over the four 16-lane groups of a wave.
 __device__ __forceinline__ float groups_max(float x) {
@@ -264,37 +212,6 @@ struct Tile {
   }
 };
 
-// Keys of a split of a row block: `keys` keys that some row sees in at most nsplit parts, each whole
-// steps of the workgroup's waves.
-__host__ __device__ __forceinline__ int split_keys(int keys, int nsplit) {
-  const int step = kWaves * kStep;
-  const int per = (keys + nsplit - 1) / nsplit;
-  return max((per + step - 1) / step * step, step);
-}
-
-// Token range of a row block, and how many keys its rows see.
-struct Block {
-  int past, fresh, r0, rows, lmin, keys;
-};
-
-__device__ __forceinline__ Block block_of(const PagedArgs& a, int b, int rb, int G) {
-  Block x;
-  x.past = past_of(a.past, b);
-  x.fresh = fresh_of(a.fresh, b, a.N);
-  x.r0 = rb * kRows;
-  x.rows = a.N * G;
-  const int tok0 = x.r0 / G, tok1 = min(min((x.r0 + kRows - 1) / G, a.N - 1), x.fresh - 1);
-  x.lmin = x.past + tok0;                              // the last key that the first live row sees
-  x.keys = tok0 < x.fresh ? x.past + tok1 + 1 : 0;
-  return x;
-}
-
-// A split leaves, for each row, D unnormalised sums, m' and l.
-template <int D>
-__device__ __forceinline__ float* part_row(const PagedArgs& a, long long block, int split, int row) {
-  return a.part + ((block * a.nsplit + split) * kRows + row) * (D + 4);
-}
-
 template <typename E, int D>
 __global__ __launch_bounds__(64 * kWaves) void attend_kernel(PagedArgs a, int row_blocks) {
   typedef Tile<D> T;
@@ -312,8 +229,8 @@ __global__ __launch_bounds__(64 * kWaves) void attend_kernel(PagedArgs a, int ro
   const long long block = blockIdx.x / a.nsplit;
   const int rb = block % row_blocks, bh = block / row_blocks;
   const int b = bh / Hkv, hk = bh % Hkv;
-  const Block x = block_of(a, b, rb, G);
-  const int per = split_keys(x.keys, a.nsplit);
+  const Block x = block_of(a, b, rb, G, kRows);
+  const int per = split_keys(x.keys, a.nsplit, kSplitStep);
   const int first = split * per, last = min(first + per, x.keys);   // keys of this workgroup
   if (split > 0 && first >= x.keys) return;                        // (the first split also writes what has no keys)
 
@@ -345,9 +262,9 @@ __global__ __launch_bounds__(64 * kWaves) void attend_kernel(PagedArgs a, int ro
     const int key = first + ((j0 + lane / 2) * kWaves + wave) * kStep + 16 * (lane & 1);
     int page = key < last ? page_of(a.cache, b, key / ps) : 0;
     const long long ph = (long long)max(page, 0) * Hkv + hk;
-    const int ke = static_cast<const uint8_t*>(a.cache.k_scale)[ph], ve = static_cast<const uint8_t*>(a.cache.v_scale)[ph];
-    my_ks = page < 0 ? __builtin_nanf("") : exp2i(ke - 127) * a.scale_log2;   // (no page: its rows become NaN)
-    my_ve = page < 0 ? 0 : ve - 127;
+    const int ke = scale_of(a.cache.k_scale, ph), ve = scale_of(a.cache.v_scale, ph);
+    my_ks = page < 0 ? __builtin_nanf("") : exp2i(ke) * a.scale_log2;   // (no page: its rows become NaN)
+    my_ve = page < 0 ? 0 : ve;
     my_page = max(page, 0);
     my_row = key % ps;
   };
@@ -355,6 +272,19 @@ __global__ __launch_bounds__(64 * kWaves) void attend_kernel(PagedArgs a, int ro
     const int page = __builtin_amdgcn_readlane(my_page, i), row = __builtin_amdgcn_readlane(my_row, i);
     t.load(kp, vp, (((long long)page * Hkv + hk) * ps + row) * D, c, g);
   };
+
+  // V^T operand of dims block y: slots j = 4 u + n are keys (u, n), the lane's dim c VB + y
+  auto v_operand = [&](const T (&t)[2], int y) __attribute__((always_inline)) {
+    u32x4 r;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const uint32_t lo = cvt_f16(t[w >> 1].v[2 * (w & 1)][y >> 2], (y & 2) != 0);
+      const uint32_t hi = cvt_f16(t[w >> 1].v[2 * (w & 1) + 1][y >> 2], (y & 2) != 0);
+      r[w] = __builtin_amdgcn_perm(hi, lo, y & 1 ? 0x07060302u : 0x05040100u);
+    }
+    return r;
+  };
+  bool nan_met = false;   // a masked step of V held a NaN
 
   auto compute = [&](T (&t)[2], int i, int k0) __attribute__((always_inline)) {
     f32x4 s[2];
@@ -369,7 +299,6 @@ __global__ __launch_bounds__(64 * kWaves) void attend_kernel(PagedArgs a, int ro
 #pragma unroll
       for (int n = 0; n < 4; ++n) s[u][n] = __builtin_fmaf(s[u][n], ks, (float)ve[u]);
     }
-    bool nan_v = false;
     if (k0 + kStep - 1 > x.lmin) {
 #pragma unroll
       for (int u = 0; u < 2; ++u)
@@ -378,9 +307,10 @@ __global__ __launch_bounds__(64 * kWaves) void attend_kernel(PagedArgs a, int ro
           const int key = k0 + 16 * u + 4 * g + n;
           if (key > lim) s[u][n] = NEG_INF;
 #pragma unroll
-          for (int w = 0; w < T::VW; ++w) {
-            if (key >= x.keys) t[u].v[n][w] = 0;       // what lies behind the last key may be anything
-            nan_v |= has_nan(t[u].v[n][w]);
+          for (int w = 0; w < T::VW; ++w) {   // what lies behind the last key may be anything
+            const uint32_t v = key >= x.keys ? 0u : t[u].v[n][w], nan = nan_bytes(v);
+            t[u].v[n][w] = without_nan(v, nan);
+            nan_met |= nan != 0;
           }
         }
     }
@@ -388,7 +318,7 @@ __global__ __launch_bounds__(64 * kWaves) void attend_kernel(PagedArgs a, int ro
                      fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
     mx = groups_max(mx);
     if (__builtin_amdgcn_ballot_w64(mx > m + kLazy)) {
-      const float mn = fmaxf(m, mx - kBelow);
+      const float mn = mx > m + kLazy ? mx - kBelow : m;   // (a row's own scores alone move it)
       const float alpha = fast_exp2(m - mn);
       m = mn;
       l *= alpha;
@@ -402,45 +332,10 @@ __global__ __launch_bounds__(64 * kWaves) void attend_kernel(PagedArgs a, int ro
       for (int n = 0; n < 4; ++n) p[u][n] = fast_exp2(s[u][n] - m);
       l = __builtin_fmaf((p[u][0] + p[u][1]) + (p[u][2] + p[u][3]), exp2i(-ve[u]), l);
     }
-    // V^T operand of dims block y: slots j = 4 u + n are keys (u, n), the lane's dim c VB + y
-    auto v_operand = [&](int y) __attribute__((always_inline)) {
-      u32x4 r;
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        const uint32_t lo = cvt_f16(t[w >> 1].v[2 * (w & 1)][y >> 2], (y & 2) != 0);
-        const uint32_t hi = cvt_f16(t[w >> 1].v[2 * (w & 1) + 1][y >> 2], (y & 2) != 0);
-        r[w] = __builtin_amdgcn_perm(hi, lo, y & 1 ? 0x07060302u : 0x05040100u);
-      }
-      return r;
-    };
     const u32x4 pf = {pack2<F16>(p[0][0], p[0][1]), pack2<F16>(p[0][2], p[0][3]), pack2<F16>(p[1][0], p[1][1]),
                       pack2<F16>(p[1][2], p[1][3])};
-    if (__builtin_amdgcn_ballot_w64(nan_v)) {
-      // A NaN in V may lie behind some row's last key, where 0 NaN would reach that row: add the
-      // other values, then make NaN what sees one: counts = seen (1 or 0) x is NaN (1 or 0).
-      u32x4 seen;
 #pragma unroll
-      for (int w = 0; w < 4; ++w)
-        seen[w] = pack2<F16>(s[w >> 1][2 * (w & 1)] == NEG_INF ? 0.f : 1.f, s[w >> 1][2 * (w & 1) + 1] == NEG_INF ? 0.f : 1.f);
-#pragma unroll
-      for (int y = 0; y < VB; ++y) {
-        u32x4 v = v_operand(y), is;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          const bool lo = (v[w] & 0x7FFFu) > 0x7C00u, hi = (v[w] & 0x7FFF0000u) > 0x7C000000u;
-          is[w] = (lo ? 0x3C00u : 0u) | (hi ? 0x3C000000u : 0u);
-          v[w] = (lo ? 0u : v[w] & 0xFFFFu) | (hi ? 0u : v[w] & 0xFFFF0000u);
-        }
-        acc[y] = mfma16<F16>(v, pf, acc[y]);
-        const f32x4 count = mfma16<F16>(is, seen, f32x4{});
-#pragma unroll
-        for (int n = 0; n < 4; ++n)
-          if (count[n] > 0.f) acc[y][n] = __builtin_nanf("");
-      }
-    } else {
-#pragma unroll
-      for (int y = 0; y < VB; ++y) acc[y] = mfma16<F16>(v_operand(y), pf, acc[y]);
-    }
+    for (int y = 0; y < VB; ++y) acc[y] = mfma16<F16>(v_operand(t, y), pf, acc[y]);
   };
 
   // The next step's bytes are on their way while a step is computed; past the last one its own
@@ -456,6 +351,35 @@ __global__ __launch_bounds__(64 * kWaves) void attend_kernel(PagedArgs a, int ro
       compute(ta, 2 * j, first + ((j0 + j) * kWaves + wave) * kStep);
       load_tile(ta[0], 2 * j2), load_tile(ta[1], 2 * j2 + 1);
       if (j + 1 < n) compute(tb, 2 * j + 2, first + ((j0 + j + 1) * kWaves + wave) * kStep);
+    }
+  }
+
+  if (__builtin_amdgcn_ballot_w64(nan_met)) {
+    for (int j = 0; j < steps; ++j) {
+      const int k0 = first + (j * kWaves + wave) * kStep;
+      if (k0 + kStep - 1 <= x.lmin || k0 >= last) continue;
+      T t[2];
+      u32x4 seen;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int key = k0 + 16 * u;
+        const long long page = key < last ? max(page_of(a.cache, b, key / ps), 0) : 0;
+        t[u].load(kp, vp, ((page * Hkv + hk) * ps + key % ps) * D, c, g);
+#pragma unroll
+        for (int n = 0; n < 4; ++n)
+#pragma unroll
+          for (int w = 0; w < T::VW; ++w) t[u].v[n][w] = key + 4 * g + n < x.keys ? nan_as_one(t[u].v[n][w]) : 0u;
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+          seen[2 * u + n] = (key + 4 * g + 2 * n <= lim ? 0x3C00u : 0u) | (key + 4 * g + 2 * n + 1 <= lim ? 0x3C000000u : 0u);
+      }
+#pragma unroll
+      for (int y = 0; y < VB; ++y) {
+        const f32x4 count = mfma16<F16>(v_operand(t, y), seen, f32x4{});
+#pragma unroll
+        for (int n = 0; n < 4; ++n)
+          if (count[n] > 0.f) acc[y][n] = __builtin_nanf("");
+      }
     }
   }
 
@@ -489,7 +413,7 @@ __global__ __launch_bounds__(64 * kWaves) void attend_kernel(PagedArgs a, int ro
     o[i] = z;
   }
   if (per < x.keys) {   // more than one split: the join divides
-    float* const dst = part_row<D>(a, block, split, row);
+    float* const dst = part_row<D>(a, block, split, row, kRows);
 #pragma unroll
     for (int i = 0; i < PER; ++i) dst[d0 + i] = o[i];
     if (d0 == 0) dst[D] = M, dst[D + 1] = L;
@@ -509,29 +433,29 @@ __global__ __launch_bounds__(64 * kWaves) void attend_kernel(PagedArgs a, int ro
 constexpr int kJoinThreads = 256;
 
 template <typename E, int D>
-__global__ __launch_bounds__(kJoinThreads) void join_kernel(PagedArgs a, int row_blocks) {
+__global__ __launch_bounds__(kJoinThreads) void join_kernel(PagedArgs a, int row_blocks, int block_rows, int step) {
   constexpr int TR = D / 4, PAR = kJoinThreads / TR;
   __shared__ float ml[kMaxSplit][2];
   __shared__ __attribute__((aligned(16))) float sums[PAR][D];
   const int Hkv = a.cache.H_kv, G = a.H / Hkv, rows = a.N * G;
   const int bh = blockIdx.x / rows, rr = blockIdx.x % rows, b = bh / Hkv, hk = bh % Hkv;
-  const Block x = block_of(a, b, rr / kRows, G);
-  const int per = split_keys(x.keys, a.nsplit);
+  const Block x = block_of(a, b, rr / block_rows, G, block_rows);
+  const int per = split_keys(x.keys, a.nsplit, step);
   if (per >= x.keys) return;
   const int n = (x.keys + per - 1) / per;
-  const long long block = (long long)bh * row_blocks + rr / kRows;
+  const long long block = (long long)bh * row_blocks + rr / block_rows;
   const int p = threadIdx.x / TR, d0 = threadIdx.x % TR * 4;
-  const float* const src = part_row<D>(a, block, 0, rr % kRows);
-  constexpr int STRIDE = kRows * (D + 4);
+  const float* const src = part_row<D>(a, block, 0, rr % block_rows, block_rows);
+  const int stride = block_rows * (D + 4);
   if (threadIdx.x < n) {
-    ml[threadIdx.x][0] = src[threadIdx.x * STRIDE + D];
-    ml[threadIdx.x][1] = src[threadIdx.x * STRIDE + D + 1];
+    ml[threadIdx.x][0] = src[threadIdx.x * stride + D];
+    ml[threadIdx.x][1] = src[threadIdx.x * stride + D + 1];
   }
   // (the sums' loads do not wait for the factors)
   constexpr int AHEAD = kMaxSplit / PAR < 8 ? kMaxSplit / PAR : 8;
   f32x4 v[AHEAD];
 #pragma unroll
-  for (int i = 0; i < AHEAD; ++i) v[i] = gload_f32x4(src + min(p + i * PAR, n - 1) * STRIDE + d0);
+  for (int i = 0; i < AHEAD; ++i) v[i] = gload_f32x4(src + min(p + i * PAR, n - 1) * stride + d0);
   __syncthreads();
   float M = -__FLT_MAX__, L = 0.f;
   for (int s = 0; s < n; ++s) M = fmaxf(M, ml[s][0]);
@@ -546,7 +470,7 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(PagedArgs a, int row
   }
   for (int s = p + AHEAD * PAR; s < n; s += PAR) {
     const float f = fast_exp2(ml[s][0] - M);
-    const f32x4 w = gload_f32x4(src + s * STRIDE + d0);
+    const f32x4 w = gload_f32x4(src + s * stride + d0);
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(f, w[e], o[e]);
   }
@@ -603,32 +527,46 @@ int launch_append(AppendArgs a) {
                            : launch_append_passes<E, D, false>(a, (int)q_blocks, q_chunks, touched, items + q_blocks);
 }
 
-// Splits of each row block's keys: enough workgroups for every CU's share of kPerCu, none with fewer keys
-// than one step of its waves.
-constexpr int kPerCu = 4;
+// How a call's rows and keys are cut: blocks of `rows` rows, each block's keys in up to nsplit parts of
+// whole `step`s, enough for kPerCu workgroups to a CU.
+struct Cut {
+  int rows, step, row_blocks, nsplit;
+};
 
-int split_of(int B, int Hkv, int row_blocks, long long keys) {
-  const long long blocks = (long long)B * Hkv * row_blocks;
-  const long long want = (kPerCu * (long long)cu_count() + blocks - 1) / blocks;
-  const long long most = (keys + kWaves * kStep - 1) / (kWaves * kStep);
-  return (int)std::max<long long>(1, std::min<long long>({want, most, kMaxSplit}));
+constexpr int kPerCu = 4, kPerCuRows = 2;
+
+Cut cut_of(int B, int H, int Hkv, int N, long long keys) {
+  Cut c;
+  const long long rows = (long long)N * (H / Hkv);
+  const bool many = rows > 64;
+  c.rows = many ? kBlockRows : kRows;
+  c.step = many ? kBlockKeys : kSplitStep;
+  c.row_blocks = (int)((rows + c.rows - 1) / c.rows);
+  const long long blocks = (long long)B * Hkv * c.row_blocks;
+  const long long want = ((many ? kPerCuRows : kPerCu) * (long long)cu_count() + blocks - 1) / blocks;
+  const long long most = many ? keys / (4 * kBlockKeys) : (keys + kSplitStep - 1) / kSplitStep;
+  c.nsplit = (int)std::max<long long>(1, std::min<long long>({want, most, kMaxSplit}));
+  return c;
 }
 
-int row_blocks_of(int N, int G) { return (int)(((long long)N * G + kRows - 1) / kRows); }
-
-size_t part_bytes(int B, int Hkv, int row_blocks, int nsplit, int D) {
-  return nsplit <= 1 ? 0 : (size_t)B * Hkv * row_blocks * nsplit * kRows * (D + 4) * sizeof(float);
+size_t part_bytes(int B, int Hkv, const Cut& c, int D) {
+  return c.nsplit <= 1 ? 0 : (size_t)B * Hkv * c.row_blocks * c.nsplit * c.rows * (D + 4) * sizeof(float);
 }
 
 template <typename E, int D>
-int launch_attend(const PagedArgs& a) {
-  const int row_blocks = row_blocks_of(a.N, a.H / a.cache.H_kv);
-  const long long grid = (long long)a.B * a.cache.H_kv * row_blocks * a.nsplit;
+int launch_attend(const PagedArgs& a, const Cut& c, int dtype) {
+  const long long grid = (long long)a.B * a.cache.H_kv * c.row_blocks * a.nsplit;
   const long long joins = (long long)a.B * a.H * a.N;
   if (grid > 0x7fffffffLL || joins > 0x7fffffffLL) return FA_ERR_DIMS;
-  hipLaunchKernelGGL((attend_kernel<E, D>), dim3((unsigned)grid), dim3(64 * kWaves), 0, (hipStream_t)a.stream, a, row_blocks);
+  hipStream_t st = (hipStream_t)a.stream;
+  if (c.rows == kRows) {
+    hipLaunchKernelGGL((attend_kernel<E, D>), dim3((unsigned)grid), dim3(64 * kWaves), 0, st, a, c.row_blocks);
+  } else {
+    const int status = paged_rows(dtype, a, c.row_blocks);
+    if (status != FA_OK) return status;
+  }
   if (a.nsplit > 1)
-    hipLaunchKernelGGL((join_kernel<E, D>), dim3((unsigned)joins), dim3(kJoinThreads), 0, (hipStream_t)a.stream, a, row_blocks);
+    hipLaunchKernelGGL((join_kernel<E, D>), dim3((unsigned)joins), dim3(kJoinThreads), 0, st, a, c.row_blocks, c.rows, c.step);
   return hipGetLastError() == hipSuccess ? FA_OK : FA_ERR_LAUNCH;
 }
 
@@ -646,22 +584,22 @@ int paged_append(int dtype, const AppendArgs& a) {
 }
 
 int paged_attention(int dtype, PagedArgs a, size_t workspace_bytes) {
-  const int Hkv = a.cache.H_kv, row_blocks = row_blocks_of(a.N, a.H / Hkv);
-  a.nsplit = split_of(a.B, Hkv, row_blocks, (long long)a.cache.table_width * a.cache.page_size);
-  while (a.nsplit > 1 && part_bytes(a.B, Hkv, row_blocks, a.nsplit, a.D) > workspace_bytes) --a.nsplit;
+  const int Hkv = a.cache.H_kv;
+  Cut c = cut_of(a.B, a.H, Hkv, a.N, (long long)a.cache.table_width * a.cache.page_size);
+  while (c.nsplit > 1 && part_bytes(a.B, Hkv, c, a.D) > workspace_bytes) --c.nsplit;
+  a.nsplit = c.nsplit;
   if (dtype == FA_BF16) {
-    if (a.D == 32) return launch_attend<BF16, 32>(a);
-    if (a.D == 64) return launch_attend<BF16, 64>(a);
-    return launch_attend<BF16, 128>(a);
+    if (a.D == 32) return launch_attend<BF16, 32>(a, c, dtype);
+    if (a.D == 64) return launch_attend<BF16, 64>(a, c, dtype);
+    return launch_attend<BF16, 128>(a, c, dtype);
   }
-  if (a.D == 32) return launch_attend<F16, 32>(a);
-  if (a.D == 64) return launch_attend<F16, 64>(a);
-  return launch_attend<F16, 128>(a);
+  if (a.D == 32) return launch_attend<F16, 32>(a, c, dtype);
+  if (a.D == 64) return launch_attend<F16, 64>(a, c, dtype);
+  return launch_attend<F16, 128>(a, c, dtype);
 }
 
 size_t paged_attention_workspace(int B, int H, int Hkv, int N, int D, long long keys) {
-  const int row_blocks = row_blocks_of(N, H / Hkv);
-  return part_bytes(B, Hkv, row_blocks, split_of(B, Hkv, row_blocks, keys), D);
+  return part_bytes(B, Hkv, cut_of(B, H, Hkv, N, keys), D);
 }
 
 }  // namespace fa

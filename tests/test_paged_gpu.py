@@ -151,6 +151,22 @@ def test_what_lies_behind_a_rows_last_key_does_not_touch_it(dt, N):
         assert torch.isnan(o[0, :, N // 2:]).all()
 
 
+@pytest.mark.parametrize("N", [1, 90])
+def test_pages_that_hold_nothing_yet(N):
+    """The tiles behind a row's last key read some page, whatever bytes its scale has (0: an empty cache's)."""
+    cache = filled(10, 2, 16, 128, 8)
+    bt = torch.arange(1, 10, device="cuda").int()[None]
+    q = randn(9, 1, 4, N, 128).bfloat16()
+    want = check_attend(q, cache, bt, ints(100 - N))
+    for byte in (0, 254, 255):
+        for t in cache[2:]:
+            t.view(torch.uint8)[0] = byte
+            t.view(torch.uint8)[9] = byte
+        cache.k.view(torch.uint8)[0] = 0x7F
+        cache.v.view(torch.uint8)[0] = 0x7F
+        assert torch.equal(fused_paged_attention(q, cache, bt, ints(100 - N)), want)
+
+
 def test_nan_in_a_value_reaches_its_dim_alone():
     cache = filled(8, 1, 16, 64, 5)
     bt = tables(1, 8, 8, 5)
