@@ -105,7 +105,7 @@ __device__ __forceinline__ float* part_row(const PagedArgs& a, long long block, 
 }
 
 // (fa_paged_rows.hip) blocks of kBlockRows rows, keys in tiles of kBlockKeys
-constexpr int kBlockRows = 128, kBlockKeys = 64;
+constexpr int kBlockRows = 256, kBlockKeys = 64;
 int paged_rows(int dtype, const PagedArgs& a, int row_blocks);
 
 }  // namespace fa

@@ -4,9 +4,9 @@
 // The matrix instructions bound it, so the codes become 16-bit values once per workgroup and not once
 // per wave: a workgroup of 4 waves takes 128 rows (32 to a wave; row r = token r / G, query head r % G
 // of one K/V head, so neighbouring rows share every key), walks the keys in tiles of 64, and keeps two
-// tiles of K (in the queries' type) and V (fp16) in LDS.  While tile j is computed, the codes of K tile
-// j + 2 and V tile j + 1 are on their way to registers; they are converted (2 codes an instruction) and
-// written to LDS behind its products.  Products, layouts and order of a step are those of the causal
+// tiles of K (in the queries' type) and V (fp16) in LDS.  A tile's codes come to registers while the tile
+// before them is computed, are converted (2 codes an instruction) and written to LDS under the products of
+// the next step, and are read in the step after it: no wave waits for them between two products.  Products, layouts and order of a step are those of the causal
 // forward (fa_fwd.hip): S^T = K Q^T on 32x32x16 products with a lane owning one row, the scores fed
 // back as the B operand of O^T += V^T P^T, V^T read transposed from LDS, S(j + 1) under the softmax of
 // S(j).  What differs:
@@ -47,6 +47,7 @@ void rows_kernel(PagedArgs a, int row_blocks) {
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane & 31, hh = lane >> 5;
   const int Hkv = a.cache.H_kv, ps = a.cache.page_size, G = a.H / Hkv;
+  const int page_bits = 31 - __builtin_clz(ps);   // (a power of two)
 
   // Workgroups reach the XCDs in turn (wg % 8): XCD x takes a contiguous range of (batch, K/V head)
   // units, so their pages stay in its L2, and of each the last rows, whose keys are the most, first.
@@ -86,20 +87,25 @@ void rows_kernel(PagedArgs a, int row_blocks) {
   // ---- pages and scales: lane i holds those of part i (16 keys) of the run of 16 tiles from run0, and of
   // the next run
   struct Parts {
-    int page, ve;
+    uint32_t lo, hi;   // offset of its first row in the pools
+    int ve;
     float ks;
   };
   Parts cur{}, nxt{};
   auto part_page = [&](int t0) __attribute__((always_inline)) {   // of the run that starts at tile t0
     const int key = first + t0 * BN + 16 * lane;
-    return key < last ? page_of(a.cache, b, key / ps) : 0;
+    return key < last ? page_of(a.cache, b, key >> page_bits) : 0;
+  };
+  auto part_place = [&](Parts& p, int t0, int page) __attribute__((always_inline)) {
+    const int key = first + t0 * BN + 16 * lane;
+    const uint64_t at = ((((uint64_t)max(page, 0) * Hkv + hk) << page_bits) + (key & (ps - 1))) * D;
+    p.lo = (uint32_t)at, p.hi = (uint32_t)(at >> 32);
   };
   auto part_scales = [&](Parts& p, int page) __attribute__((always_inline)) {
     const long long ph = (long long)max(page, 0) * Hkv + hk;
     const int ke = scale_of(a.cache.k_scale, ph), ve = scale_of(a.cache.v_scale, ph);
     p.ks = page < 0 ? __builtin_nanf("") : exp2i(ke) * a.scale_log2;   // (no page: its rows become NaN)
     p.ve = page < 0 ? 0 : ve;
-    p.page = max(page, 0);
   };
   int run0 = 0;
 
@@ -112,11 +118,13 @@ void rows_kernel(PagedArgs a, int row_blocks) {
   const int vdst = prow * ROWB + ((tid % PCR * 32) ^ ((32 * (prow & 3)) & (ROWB - 1)));
   const bool stages = PIECES >= NT || tid < PIECES;
   auto fetch = [&](const void* pool, int t, u32x4 (&w)[PT]) __attribute__((always_inline)) {
-    const int mine = t - run0 < 16 ? cur.page : nxt.page;
+    const uint32_t lo = t - run0 < 16 ? cur.lo : nxt.lo, hi = t - run0 < 16 ? cur.hi : nxt.hi;
     // a piece's row lies in part prow / 16, the same for a whole wave (D = 32: for half a wave)
     auto part = [&](int i) __attribute__((always_inline)) {
-      const int page = __builtin_amdgcn_readlane(mine, ((t - run0) & 15) * 4 + i);
-      return static_cast<const uint8_t*>(pool) + (((long long)page * Hkv + hk) * ps + (first + t * BN + 16 * i) % ps) * D;
+      const int from = ((t - run0) & 15) * 4 + i;
+      const uint64_t at = (uint64_t)(uint32_t)__builtin_amdgcn_readlane(hi, from) << 32 |
+                          (uint32_t)__builtin_amdgcn_readlane(lo, from);
+      return static_cast<const uint8_t*>(pool) + at;
     };
 #pragma unroll
     for (int i = 0; i < PT; ++i) {
@@ -130,13 +138,22 @@ void rows_kernel(PagedArgs a, int row_blocks) {
       w[i] = *reinterpret_cast<const u32x4*>(p + goff);
     }
   };
-  auto put_k = [&](const u32x4 (&w)[PT], unsigned char* buf) __attribute__((always_inline)) {
-    if (!stages) return;
+  // (a 16-byte write serves 8 lanes at a time over 128 bytes of banks: with every other four lanes' halves
+  // swapped those 8 pieces, 32 bytes apart, meet 8 different sixteenths)
+  const bool upper = (tid & 4) != 0;
+  const int half0 = upper ? 16 : 0;
+  auto put_as = [&](auto type, const u32x4 (&w)[PT], int dst, unsigned char* buf) __attribute__((always_inline)) {
+    typedef decltype(type) T;
 #pragma unroll
     for (int i = 0; i < PT; ++i) {
-      lds_write16(buf, kdst + i * RP * ROWB, codes8<E>(w[i][0], w[i][1]));
-      lds_write16(buf, (kdst ^ 16) + i * RP * ROWB, codes8<E>(w[i][2], w[i][3]));
+      const u32x4 x = upper ? u32x4{w[i][2], w[i][3], w[i][0], w[i][1]} : w[i];
+      lds_write16(buf, (dst ^ half0) + i * RP * ROWB, codes8<T>(x[0], x[1]));
+      lds_write16(buf, (dst ^ half0 ^ 16) + i * RP * ROWB, codes8<T>(x[2], x[3]));
     }
+  };
+  auto put_k = [&](const u32x4 (&w)[PT], unsigned char* buf) __attribute__((always_inline)) {
+    if (!stages) return;
+    put_as(E{}, w, kdst, buf);
   };
   auto put_v = [&](u32x4 (&w)[PT], int t, unsigned char* buf, auto full) __attribute__((always_inline)) {
     if (!stages) return;
@@ -153,11 +170,7 @@ void rows_kernel(PagedArgs a, int row_blocks) {
         if (any != 0) nan_met = 1;
       }
     }
-#pragma unroll
-    for (int i = 0; i < PT; ++i) {
-      lds_write16(buf, vdst + i * RP * ROWB, codes8<F16>(w[i][0], w[i][1]));
-      lds_write16(buf, (vdst ^ 16) + i * RP * ROWB, codes8<F16>(w[i][2], w[i][3]));
-    }
+    put_as(F16{}, w, vdst, buf);
   };
 
   // ---- per-lane LDS operand offsets (fa_fwd.hip)
@@ -279,8 +292,9 @@ void rows_kernel(PagedArgs a, int row_blocks) {
 
   if (ntiles > 0) {
     if (tid == 0) nan_met = 0;
-    part_scales(cur, part_page(0));
-    int nxt_page = 0;
+    int nxt_page = part_page(0);
+    part_place(cur, 0, nxt_page);
+    part_scales(cur, nxt_page);
     u32x4 rk[PT], rv[PT];
     __syncthreads();
     fetch(a.cache.k, 0, rk);
@@ -292,6 +306,8 @@ void rows_kernel(PagedArgs a, int row_blocks) {
       put_k(rk, Kbuf(1));
     }
     __syncthreads();
+    fetch(a.cache.k, 2, rk);
+    fetch(a.cache.v, 1, rv);
     f32x16 sa[NB], sb[NB];
     s_tile(Kbuf(0), sa);
     if (jfull == 0) mask_tile(sa, first);
@@ -301,24 +317,24 @@ void rows_kernel(PagedArgs a, int row_blocks) {
                     const unsigned char* __restrict__ vcur, unsigned char* __restrict__ vdst_, f32x16 (&sc)[NB],
                     f32x16 (&sn)[NB], auto full) __attribute__((always_inline)) {
       constexpr bool FULL = decltype(full)::value;
-      const bool more = FULL || j + 2 < ntiles;
-      if (more) fetch(a.cache.k, j + 2, rk);
-      fetch(a.cache.v, j + 1, rv);
+      // (past the last tile what is written is not read, and what is fetched lies in some page)
+      put_k(rk, kdst_);
+      put_v(rv, j + 1, vdst_, full);
+      fetch(a.cache.k, j + 3, rk);
+      fetch(a.cache.v, j + 2, rv);
       u32x4 pk[2 * NB];
       s_tile(kcur, sn);
       if constexpr (!FULL) mask_tile(sn, first + (j + 1) * BN);
       pv_pre(vcur);
       softmax(sc, j, pk);
       pv_full(vcur, pk);
-      if (more) put_k(rk, kdst_);
-      put_v(rv, j + 1, vdst_, full);
     };
     auto iteration = [&](int j, f32x16 (&sc)[NB], f32x16 (&sn)[NB], auto full) __attribute__((always_inline)) {
       // a run's pages are asked for at its predecessor's start, their scales half a run later
       if ((j & 15) == 0) {
         if (j > 0) cur = nxt, run0 = j;
         nxt_page = part_page(j + 16);
-        nxt.page = max(nxt_page, 0);
+        part_place(nxt, j + 16, nxt_page);
       } else if ((j & 15) == 8) {
         part_scales(nxt, nxt_page);
       }
@@ -350,8 +366,8 @@ void rows_kernel(PagedArgs a, int row_blocks) {
 #pragma unroll
         for (int i = 0; i < PT; ++i) {
           const int key = first + t * BN + prow + i * RP;
-          const long long page = key < x.keys ? max(page_of(a.cache, b, key / ps), 0) : 0;
-          const uint8_t* const p = static_cast<const uint8_t*>(a.cache.v) + ((page * Hkv + hk) * ps + key % ps) * D + tid % PCR * 16;
+          const long long page = key < x.keys ? max(page_of(a.cache, b, key >> page_bits), 0) : 0;
+          const uint8_t* const p = static_cast<const uint8_t*>(a.cache.v) + ((page * Hkv + hk) * ps + (key & (ps - 1))) * D + tid % PCR * 16;
           const u32x4 w = *reinterpret_cast<const u32x4*>(p);
 #pragma unroll
           for (int n = 0; n < 4; ++n) rv[i][n] = key < x.keys ? nan_as_one(w[n]) : 0u;
