@@ -104,8 +104,8 @@ __device__ __forceinline__ float* part_row(const PagedArgs& a, long long block, 
   return a.part + ((block * a.nsplit + split) * block_rows + row) * (D + 4);
 }
 
-// (fa_paged_rows.hip) blocks of kBlockRows rows, keys in tiles of kBlockKeys
-constexpr int kBlockRows = 256, kBlockKeys = 64;
-int paged_rows(int dtype, const PagedArgs& a, int row_blocks);
+// (fa_paged_rows.hip) blocks of 128 or 256 rows, keys in tiles of kBlockKeys
+constexpr int kBlockKeys = 64;
+int paged_rows(int dtype, const PagedArgs& a, int row_blocks, int block_rows);
 
 }  // namespace fa

@@ -435,7 +435,7 @@ constexpr int kJoinThreads = 256;
 template <typename E, int D>
 __global__ __launch_bounds__(kJoinThreads) void join_kernel(PagedArgs a, int row_blocks, int block_rows, int step) {
   constexpr int TR = D / 4, PAR = kJoinThreads / TR;
-  __shared__ float ml[kMaxSplit][2];
+  __shared__ float factor[kMaxSplit];
   __shared__ __attribute__((aligned(16))) float sums[PAR][D];
   const int Hkv = a.cache.H_kv, G = a.H / Hkv, rows = a.N * G;
   const int bh = blockIdx.x / rows, rr = blockIdx.x % rows, b = bh / Hkv, hk = bh % Hkv;
@@ -447,32 +447,43 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(PagedArgs a, int row
   const int p = threadIdx.x / TR, d0 = threadIdx.x % TR * 4;
   const float* const src = part_row<D>(a, block, 0, rr % block_rows, block_rows);
   const int stride = block_rows * (D + 4);
-  if (threadIdx.x < n) {
-    ml[threadIdx.x][0] = src[threadIdx.x * stride + D];
-    ml[threadIdx.x][1] = src[threadIdx.x * stride + D + 1];
+  // every wave takes the maximum and the sum of all (m', l), two splits to a lane; the first keeps the factors
+  const int lane = threadIdx.x & 63;
+  float m[2], l[2], M = -__FLT_MAX__, L = 0.f;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const float* const ml = src + min(lane + 64 * i, n - 1) * stride + D;
+    m[i] = ml[0], l[i] = lane + 64 * i < n ? ml[1] : 0.f;
   }
   // (the sums' loads do not wait for the factors)
   constexpr int AHEAD = kMaxSplit / PAR < 8 ? kMaxSplit / PAR : 8;
   f32x4 v[AHEAD];
 #pragma unroll
   for (int i = 0; i < AHEAD; ++i) v[i] = gload_f32x4(src + min(p + i * PAR, n - 1) * stride + d0);
+  M = fmaxf(m[0], m[1]);
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) M = fmaxf(M, __shfl_xor(M, d));
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const float f = fast_exp2(m[i] - M);
+    L = __builtin_fmaf(f, l[i], L);
+    if (threadIdx.x < 64) factor[lane + 64 * i] = lane + 64 * i < n ? f : 0.f;
+  }
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) L += __shfl_xor(L, d);
   __syncthreads();
-  float M = -__FLT_MAX__, L = 0.f;
-  for (int s = 0; s < n; ++s) M = fmaxf(M, ml[s][0]);
-  for (int s = 0; s < n; ++s) L = __builtin_fmaf(fast_exp2(ml[s][0] - M), ml[s][1], L);
   f32x4 o = f32x4{};
 #pragma unroll
   for (int i = 0; i < AHEAD; ++i) {
     const int s = p + i * PAR;
-    const float f = s < n ? fast_exp2(ml[s][0] - M) : 0.f;
+    const float f = s < n ? factor[s] : 0.f;
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[e] = s < n ? __builtin_fmaf(f, v[i][e], o[e]) : o[e];
   }
   for (int s = p + AHEAD * PAR; s < n; s += PAR) {
-    const float f = fast_exp2(ml[s][0] - M);
     const f32x4 w = gload_f32x4(src + s * stride + d0);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(f, w[e], o[e]);
+    for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(factor[s], w[e], o[e]);
   }
   *reinterpret_cast<f32x4*>(&sums[p][d0]) = o;
   __syncthreads();
@@ -489,6 +500,51 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(PagedArgs a, int row
   uint16_t* dst = static_cast<uint16_t*>(const_cast<void*>(a.o.data)) + b * a.o.stride_b + oh * a.o.stride_h + ot * a.o.stride_n;
   *reinterpret_cast<uint32_t*>(dst + 2 * threadIdx.x) = live ? pack2<E>(z[0] * inv, z[1] * inv) : 0u;
   if (a.lse != nullptr && threadIdx.x == 0)
+    a.lse[((long long)b * a.H + oh) * a.N + ot] = live ? M + __log2f(L) : -__builtin_inff();
+}
+
+// The same for few splits and many rows: D / 4 threads to a row, which walk its splits.
+constexpr int kFewSplits = 16;
+
+template <typename E, int D>
+__global__ __launch_bounds__(kJoinThreads) void join_few_kernel(PagedArgs a, int row_blocks, int block_rows, int step) {
+  constexpr int TR = D / 4;
+  const int Hkv = a.cache.H_kv, G = a.H / Hkv, rows = a.N * G;
+  const long long i = (long long)blockIdx.x * (kJoinThreads / TR) + threadIdx.x / TR;   // (batch, K/V head), row
+  if (i >= (long long)a.B * Hkv * rows) return;
+  const int bh = i / rows, rr = i % rows, b = bh / Hkv, hk = bh % Hkv;
+  const Block x = block_of(a, b, rr / block_rows, G, block_rows);
+  const int per = split_keys(x.keys, a.nsplit, step);
+  if (per >= x.keys) return;
+  const int n = (x.keys + per - 1) / per;
+  const float* const src = part_row<D>(a, (long long)bh * row_blocks + rr / block_rows, 0, rr % block_rows, block_rows);
+  const int stride = block_rows * (D + 4), d0 = threadIdx.x % TR * 4;
+  float m[kFewSplits], l[kFewSplits], M = -__FLT_MAX__, L = 0.f;
+  f32x4 v[kFewSplits], o = f32x4{};
+#pragma unroll
+  for (int s = 0; s < kFewSplits; ++s)
+    if (s < n) {
+      m[s] = src[s * stride + D], l[s] = src[s * stride + D + 1];
+      v[s] = gload_f32x4(src + s * stride + d0);
+    }
+#pragma unroll
+  for (int s = 0; s < kFewSplits; ++s)
+    if (s < n) M = fmaxf(M, m[s]);
+#pragma unroll
+  for (int s = 0; s < kFewSplits; ++s)
+    if (s < n) {
+      const float f = fast_exp2(m[s] - M);
+      L = __builtin_fmaf(f, l[s], L);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(f, v[s][e], o[e]);
+    }
+  const int ot = rr / G, oh = hk * G + rr % G;
+  const bool live = ot < x.fresh;
+  const float inv = live ? 1.0f / L : 0.f;
+  uint16_t* dst = static_cast<uint16_t*>(const_cast<void*>(a.o.data)) + b * a.o.stride_b + oh * a.o.stride_h + ot * a.o.stride_n;
+  *reinterpret_cast<u32x2*>(dst + d0) =
+      live ? u32x2{pack2<E>(o[0] * inv, o[1] * inv), pack2<E>(o[2] * inv, o[3] * inv)} : u32x2{};
+  if (a.lse != nullptr && d0 == 0)
     a.lse[((long long)b * a.H + oh) * a.N + ot] = live ? M + __log2f(L) : -__builtin_inff();
 }
 
@@ -528,24 +584,44 @@ int launch_append(AppendArgs a) {
 }
 
 // How a call's rows and keys are cut: blocks of `rows` rows, each block's keys in up to nsplit parts of
-// whole `step`s, enough for kPerCu workgroups to a CU.
+// whole `step`s.  Only the lengths' bound (the table's width) is known here; a shorter sequence takes
+// fewer parts (split_keys).
 struct Cut {
   int rows, step, row_blocks, nsplit;
 };
 
-constexpr int kPerCu = 4, kPerCuRows = 2;
-
-Cut cut_of(int B, int H, int Hkv, int N, long long keys) {
+// Few rows: as many parts as give each CU a workgroup (more only divide the same bytes into shorter runs
+// and more partial rows: us at 1 / 2 / 4 workgroups to a CU, 8 sequences of 1335 to 4005 keys, 8 K/V heads, D = 128:
+// 17.4 / 20.7 / 26.4; 64 of 667 to 2000 keys 36.1 / 36.2 / 40.8; one of 16000 keys 13.8 / 15.5 / 24.9), up to
+// four where a part keeps 4096 keys, for lengths that differ (32 sequences of 5461 to 16384 keys 140.9 / 141.9 / 135.3).
+// Many rows: 32 rows go to the kernel of few rows, 128 to 128-row workgroups, more to 256-row ones (us of 16 /
+// 128 / 256 rows; 8 sequences of 4000 keys, 8 K/V heads, D = 128: 32 rows 28 / 32 / 40, 64 rows 38 / 35 / 42, 128 rows
+// 59 / 40 / 46, 256 rows 96 / 60 / 58, 512 rows 199 / 93 / 91), and the parts are those of the least cost by the
+// times that a tile of one workgroup to a CU, a workgroup's start and the join of its partial rows take.
+Cut cut_of(int B, int H, int Hkv, int N, int D, long long keys) {
   Cut c;
-  const long long rows = (long long)N * (H / Hkv);
-  const bool many = rows > 64;
-  c.rows = many ? kBlockRows : kRows;
-  c.step = many ? kBlockKeys : kSplitStep;
+  const long long rows = (long long)N * (H / Hkv), units = (long long)B * Hkv;
+  c.rows = rows <= 32 ? kRows : rows <= 128 ? 128 : 256;
   c.row_blocks = (int)((rows + c.rows - 1) / c.rows);
-  const long long blocks = (long long)B * Hkv * c.row_blocks;
-  const long long want = ((many ? kPerCuRows : kPerCu) * (long long)cu_count() + blocks - 1) / blocks;
-  const long long most = many ? keys / (4 * kBlockKeys) : (keys + kSplitStep - 1) / kSplitStep;
-  c.nsplit = (int)std::max<long long>(1, std::min<long long>({want, most, kMaxSplit}));
+  const long long blocks = units * c.row_blocks, cus = cu_count();
+  if (c.rows == kRows) {
+    c.step = kSplitStep;
+    const long long fill = (cus + blocks - 1) / blocks, four = (4 * cus + blocks - 1) / blocks;
+    c.nsplit = (int)std::max<long long>(1, std::min<long long>({std::max(fill, std::min(four, keys / 4096)),
+                                                                (keys + c.step - 1) / c.step, kMaxSplit}));
+    return c;
+  }
+  c.step = kBlockKeys;
+  const long long tiles = (keys + kBlockKeys - 1) / kBlockKeys;
+  const float tile_us = (c.rows == 128 ? 1.7f : 2.2f) * (D + 32) / 160.f;
+  float best = 0.f;
+  c.nsplit = 1;
+  for (int n = 1; n <= kMaxSplit && n <= tiles; n += n < 16 ? 1 : 8) {
+    const long long rounds = (blocks * n + cus - 1) / cus;
+    const float join = n == 1 ? 0.f : 3.f + 8e-6f / 3.f * (float)(units * rows) * (float)D * (float)n;
+    const float us = (float)rounds * (2.f + tile_us * (float)((tiles + n - 1) / n)) + join;
+    if (n == 1 || us < best) best = us, c.nsplit = n;
+  }
   return c;
 }
 
@@ -562,11 +638,14 @@ int launch_attend(const PagedArgs& a, const Cut& c, int dtype) {
   if (c.rows == kRows) {
     hipLaunchKernelGGL((attend_kernel<E, D>), dim3((unsigned)grid), dim3(64 * kWaves), 0, st, a, c.row_blocks);
   } else {
-    const int status = paged_rows(dtype, a, c.row_blocks);
+    const int status = paged_rows(dtype, a, c.row_blocks, c.rows);
     if (status != FA_OK) return status;
   }
-  if (a.nsplit > 1)
+  if (a.nsplit > kFewSplits)
     hipLaunchKernelGGL((join_kernel<E, D>), dim3((unsigned)joins), dim3(kJoinThreads), 0, st, a, c.row_blocks, c.rows, c.step);
+  else if (a.nsplit > 1)
+    hipLaunchKernelGGL((join_few_kernel<E, D>), dim3((unsigned)((joins + 1024 / D - 1) / (1024 / D))), dim3(kJoinThreads), 0,
+                       st, a, c.row_blocks, c.rows, c.step);
   return hipGetLastError() == hipSuccess ? FA_OK : FA_ERR_LAUNCH;
 }
 
@@ -585,7 +664,7 @@ int paged_append(int dtype, const AppendArgs& a) {
 
 int paged_attention(int dtype, PagedArgs a, size_t workspace_bytes) {
   const int Hkv = a.cache.H_kv;
-  Cut c = cut_of(a.B, a.H, Hkv, a.N, (long long)a.cache.table_width * a.cache.page_size);
+  Cut c = cut_of(a.B, a.H, Hkv, a.N, a.D, (long long)a.cache.table_width * a.cache.page_size);
   while (c.nsplit > 1 && part_bytes(a.B, Hkv, c, a.D) > workspace_bytes) --c.nsplit;
   a.nsplit = c.nsplit;
   if (dtype == FA_BF16) {
@@ -599,7 +678,7 @@ int paged_attention(int dtype, PagedArgs a, size_t workspace_bytes) {
 }
 
 size_t paged_attention_workspace(int B, int H, int Hkv, int N, int D, long long keys) {
-  return part_bytes(B, Hkv, cut_of(B, H, Hkv, N, keys), D);
+  return part_bytes(B, Hkv, cut_of(B, H, Hkv, N, D, keys), D);
 }
 
 }  // namespace fa

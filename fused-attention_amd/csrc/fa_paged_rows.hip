@@ -426,24 +426,25 @@ void rows_kernel(PagedArgs a, int row_blocks) {
 namespace {
 
 template <typename E, int D>
-int launch_rows(const PagedArgs& a, int row_blocks) {
-  const long long grid = (long long)a.B * a.cache.H_kv * row_blocks * a.nsplit;
-  hipLaunchKernelGGL((rows_kernel<E, D, kBlockRows / 32>), dim3((unsigned)grid), dim3(2 * kBlockRows), 0,
-                     (hipStream_t)a.stream, a, row_blocks);
+int launch_rows(const PagedArgs& a, int row_blocks, int block_rows) {
+  const dim3 g((unsigned)((long long)a.B * a.cache.H_kv * row_blocks * a.nsplit)), t(2 * block_rows);
+  hipStream_t st = (hipStream_t)a.stream;
+  if (block_rows == 128) hipLaunchKernelGGL((rows_kernel<E, D, 4>), g, t, 0, st, a, row_blocks);
+  else hipLaunchKernelGGL((rows_kernel<E, D, 8>), g, t, 0, st, a, row_blocks);
   return hipGetLastError() == hipSuccess ? FA_OK : FA_ERR_LAUNCH;
 }
 
 }  // namespace
 
-int paged_rows(int dtype, const PagedArgs& a, int row_blocks) {
+int paged_rows(int dtype, const PagedArgs& a, int row_blocks, int block_rows) {
   if (dtype == FA_BF16) {
-    if (a.D == 32) return launch_rows<BF16, 32>(a, row_blocks);
-    if (a.D == 64) return launch_rows<BF16, 64>(a, row_blocks);
-    return launch_rows<BF16, 128>(a, row_blocks);
+    if (a.D == 32) return launch_rows<BF16, 32>(a, row_blocks, block_rows);
+    if (a.D == 64) return launch_rows<BF16, 64>(a, row_blocks, block_rows);
+    return launch_rows<BF16, 128>(a, row_blocks, block_rows);
   }
-  if (a.D == 32) return launch_rows<F16, 32>(a, row_blocks);
-  if (a.D == 64) return launch_rows<F16, 64>(a, row_blocks);
-  return launch_rows<F16, 128>(a, row_blocks);
+  if (a.D == 32) return launch_rows<F16, 32>(a, row_blocks, block_rows);
+  if (a.D == 64) return launch_rows<F16, 64>(a, row_blocks, block_rows);
+  return launch_rows<F16, 128>(a, row_blocks, block_rows);
 }
 
 }  // namespace fa
