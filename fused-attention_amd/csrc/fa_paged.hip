@@ -16,20 +16,14 @@ __device__ __forceinline__ int scale_exponent(float amax) {
   return min(max(e, kScaleMin), kScaleMax);
 }
 
-// 8 values times `mul` as e4m3, to nearest even; past 448 to 448, infinities and NaN to NaN.
+// 8 values times `mul` as e4m3, to nearest even (NaN to NaN; the caller sees to it that none passes 448).
 __device__ __forceinline__ u32x2 encode8(const float (&y)[8], float mul) {
-  float z[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float x = y[i] * mul;
-    z[i] = __builtin_fabsf(y[i]) < __builtin_inff() ? __builtin_amdgcn_fmed3f(x, -kCodeMax, kCodeMax) : __builtin_nanf("");
-  }
   u32x2 r;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     int w = 0;
-    w = __builtin_amdgcn_cvt_pk_fp8_f32(z[4 * i], z[4 * i + 1], w, false);
-    w = __builtin_amdgcn_cvt_pk_fp8_f32(z[4 * i + 2], z[4 * i + 3], w, true);
+    w = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * i] * mul, y[4 * i + 1] * mul, w, false);
+    w = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * i + 2] * mul, y[4 * i + 3] * mul, w, true);
     r[i] = (uint32_t)w;
   }
   return r;
@@ -44,18 +38,20 @@ __device__ __forceinline__ void decode8(const u32x2& w, float (&y)[8]) {
 }
 
 // ---------------------------------------------------------------------------
-// Append.  The first q_blocks workgroups turn the queries (turn_heads); each of the others owns one
-// page of one sequence and K/V head, for K or for V, so nobody else writes its codes and scale: it
-// holds the page's new rows in registers, reduces their largest value, and writes codes. PASSES: rows
-// of a page over the rows that the workgroup holds at once.
-template <typename E, int D, bool INTER, int PASSES>
-__global__ __launch_bounds__(kRowThreads) void append_kernel(AppendArgs a, int q_blocks, int q_chunks, int touched) {
-  using S = Slot<D>;
+// Append.  The first `items` workgroups each own one page of one sequence and K/V head, for K or for V, so
+// nobody else writes its codes and scale: it holds the page's new rows in registers, reduces their largest
+// value, and writes codes.  The others turn the queries (turn_heads); the pages, whose chain of waits is
+// longer, go first (queries first: +3 % at B=2 H=32 H_kv=8 N=8192 D=128, +5 % at N=1).  PASSES: rows of a page
+// over the rows that the workgroup holds at once; four at most, or the registers leave too few waves (128-row
+// pages at D = 128: eight passes of 256 threads 101 us, four of 512 95; 64-row pages: four of 256 90, two of 512 91).
+template <typename E, int D, bool INTER, int PASSES, int NT>
+__global__ __launch_bounds__(NT) void append_kernel(AppendArgs a, int items, int q_chunks, int touched) {
+  using S = Slot<D, NT>;
   const int slot = threadIdx.x / S::TPR;
   const int Hkv = a.cache.H_kv, ps = a.cache.page_size;
-  if ((int)blockIdx.x < q_blocks) {
-    const int chunk = blockIdx.x % q_chunks;
-    const long long at = (long long)(blockIdx.x / q_chunks) * S::TOKENS + slot;
+  if ((int)blockIdx.x >= items) {
+    const int chunk = (blockIdx.x - items) % q_chunks;
+    const long long at = (long long)((blockIdx.x - items) / q_chunks) * S::TOKENS + slot;
     const bool valid = at < a.B * a.N;
     const int t = valid ? (int)at : 0;
     const int b = t / a.N, n = t % a.N, h0 = chunk * a.heads;
@@ -63,7 +59,7 @@ __global__ __launch_bounds__(kRowThreads) void append_kernel(AppendArgs a, int q
                             min(h0 + a.heads, a.H), valid);
     return;
   }
-  int item = blockIdx.x - q_blocks;
+  int item = blockIdx.x;
   const int h = item % Hkv;
   item /= Hkv;
   const bool is_k = item % 2 == 0;
@@ -86,61 +82,86 @@ __global__ __launch_bounds__(kRowThreads) void append_kernel(AppendArgs a, int q
   const Rows& in = is_k ? a.k : a.v;
   const uint16_t* src = static_cast<const uint16_t*>(in.data) + b * in.stride_b + h * in.stride_h + d0;
 
-  float y[PASSES][8], own[8], other[8];
+  // A row is z r: r (the norm's 1 / rms) is one factor for the row, so the largest value takes it once, and the
+  // codes take it with the scale (a power of two, so the product rounds as z r does).
+  float z[PASSES][8], r[PASSES], own[8], other[8];
   float amax = 0.f;
   if (is_k) load_weights<INTER>(a.rot, a.rot.k_weight, d0, own, other);
-  auto pass = [&](int p, float (&z)[8]) __attribute__((always_inline)) {
+  auto live = [&](int p) __attribute__((always_inline)) {
     const int n = first + p * S::TOKENS + slot - past;
-    const bool live = p * S::TOKENS + slot < ps && n >= 0 && n < fresh;
-    const int nn = live ? n : 0;
-    const u32x4 w = gload16(src + nn * in.stride_n);
+    return p * S::TOKENS + slot < ps && n >= 0 && n < fresh;
+  };
+  auto pass = [&](int p, bool all) __attribute__((always_inline)) {
+    const bool mine = all || live(p);
+    const int n = mine ? first + p * S::TOKENS + slot - past : 0;
+    const u32x4 w = gload16(src + n * in.stride_n);
+    r[p] = 1.f;
     if (is_k) {
       Turn<D, INTER> turn;
-      turn.load(a.rot, lane, d0, b, nn, (long long)past + nn);
+      turn.load(a.rot, lane, d0, b, n, (long long)past + n);
       float cw[8], sw[8];
       fold_weights(turn, own, other, cw, sw);
-      turn_row<E, D, INTER>(w, turn.fetch(w), cw, sw, a.rot.k_weight != nullptr, a.rot.eps, z);
+      r[p] = turn_row<E, D, INTER>(w, turn.fetch(w), cw, sw, a.rot.k_weight != nullptr, a.rot.eps, z[p]);
     } else {
-      unpack8<E>(w, z);
+      unpack8<E>(w, z[p]);
     }
+    float top = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float x = __builtin_fabsf(z[i]);
-      if (live && x < __builtin_inff()) amax = fmaxf(amax, x);
-    }
+    for (int i = 0; i < 8; ++i) top = fmaxf(top, __builtin_fabsf(z[p][i]));   // (NaN counts for nothing)
+    if (mine) amax = fmaxf(amax, top * r[p]);
   };
   // (a page of which a few rows are new skips the passes without one; all new, no branch parts their loads)
-  if (held == 0 && first + ps <= past + fresh) {
+  const bool all = held == 0 && first + ps <= past + fresh && ps >= S::TOKENS;
+  if (all) {
 #pragma unroll
-    for (int p = 0; p < PASSES; ++p) pass(p, y[p]);
+    for (int p = 0; p < PASSES; ++p) pass(p, true);
   } else {
 #pragma unroll
     for (int p = 0; p < PASSES; ++p) {
       const int n = first + p * S::TOKENS - past;
-      if (n + S::TOKENS > 0 && n < fresh) pass(p, y[p]);
+      if (n + S::TOKENS > 0 && n < fresh) pass(p, false);
     }
   }
+  __shared__ float tops[NT / 64];
+  auto over_all = [&](float x) __attribute__((always_inline)) {
 #pragma unroll
-  for (int m = 1; m < 64; m *= 2) amax = fmaxf(amax, __shfl_xor(amax, m));
-  __shared__ float top[kRowThreads / 64];
-  if (lane == 0) top[threadIdx.x / 64] = amax;
-  __syncthreads();
+    for (int m = 1; m < 64; m *= 2) x = fmaxf(x, __shfl_xor(x, m));
+    if (lane == 0) tops[threadIdx.x / 64] = x;
+    __syncthreads();
 #pragma unroll
-  for (int i = 0; i < kRowThreads / 64; ++i) amax = fmaxf(amax, top[i]);
+    for (int i = 0; i < NT / 64; ++i) x = fmaxf(x, tops[i]);
+    return x;
+  };
+  amax = over_all(amax);
+  if (amax > kCodeMax * exp2i(kScaleMax)) {
+    // infinities become NaN and count for nothing, finite values past the scales' range become its end
+    amax = 0.f;
+#pragma unroll
+    for (int p = 0; p < PASSES; ++p) {
+      const float end = kCodeMax * exp2i(kScaleMax);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float y = z[p][i] * r[p];
+        z[p][i] = __builtin_fabsf(y) < __builtin_inff() ? fminf(fmaxf(y, -end), end) : __builtin_nanf("");
+        if (live(p) && __builtin_fabsf(y) < __builtin_inff()) amax = fmaxf(amax, __builtin_fabsf(z[p][i]));
+      }
+      r[p] = 1.f;
+    }
+    __syncthreads();
+    amax = over_all(amax);
+  }
   int e = scale_exponent(amax);
   if (held > 0) e = max(e, e_held);
   const float mul = exp2i(-e);
 #pragma unroll
-  for (int p = 0; p < PASSES; ++p) {
-    const int row = p * S::TOKENS + slot, n = first + row - past;
-    if (row < ps && n >= 0 && n < fresh) *reinterpret_cast<u32x2*>(codes + row * D) = encode8(y[p], mul);
-  }
+  for (int p = 0; p < PASSES; ++p)
+    if (all || live(p)) *reinterpret_cast<u32x2*>(codes + (p * S::TOKENS + slot) * D) = encode8(z[p], r[p] * mul);
   if (held > 0 && e > e_held) {
     const float move = exp2i(e_held - e);
     for (int row = slot; row < held; row += S::TOKENS) {
-      float z[8];
-      decode8(*reinterpret_cast<const u32x2*>(codes + row * D), z);
-      *reinterpret_cast<u32x2*>(codes + row * D) = encode8(z, move);
+      float x[8];
+      decode8(*reinterpret_cast<const u32x2*>(codes + row * D), x);
+      *reinterpret_cast<u32x2*>(codes + row * D) = encode8(x, move);
     }
   }
   if (threadIdx.x == 0) static_cast<uint8_t*>(scales)[ph] = (uint8_t)(e + 127);
@@ -551,36 +572,38 @@ __global__ __launch_bounds__(kJoinThreads) void join_few_kernel(PagedArgs a, int
 // ---------------------------------------------------------------------------
 namespace {
 
-template <typename E, int D, bool INTER>
-int launch_append_passes(const AppendArgs& a, int q_blocks, int q_chunks, int touched, long long grid) {
-  const dim3 g((unsigned)grid), t(kRowThreads);
-  hipStream_t st = (hipStream_t)a.stream;
-  const int passes = std::max(1, a.cache.page_size / Slot<D>::TOKENS);
-  if (passes == 1) hipLaunchKernelGGL((append_kernel<E, D, INTER, 1>), g, t, 0, st, a, q_blocks, q_chunks, touched);
-  else if (passes == 2) hipLaunchKernelGGL((append_kernel<E, D, INTER, 2>), g, t, 0, st, a, q_blocks, q_chunks, touched);
-  else if constexpr (D >= 64) {
-    if (passes == 4) hipLaunchKernelGGL((append_kernel<E, D, INTER, 4>), g, t, 0, st, a, q_blocks, q_chunks, touched);
-    else if constexpr (D >= 128) hipLaunchKernelGGL((append_kernel<E, D, INTER, 8>), g, t, 0, st, a, q_blocks, q_chunks, touched);
-  }
-  return hipGetLastError() == hipSuccess ? FA_OK : FA_ERR_LAUNCH;
-}
-
-template <typename E, int D>
+template <typename E, int D, bool INTER, int PASSES, int NT>
 int launch_append(AppendArgs a) {
+  typedef Slot<D, NT> S;
   const int ps = a.cache.page_size, touched = (a.N + ps - 2) / ps + 1;
   const long long items = 2LL * a.B * touched * a.cache.H_kv;
   long long q_blocks = 0;
   int q_chunks = 0;
   if (a.q.data != nullptr) {
-    const long long token_blocks = ((long long)a.B * a.N + Slot<D>::TOKENS - 1) / Slot<D>::TOKENS;
+    const long long token_blocks = ((long long)a.B * a.N + S::TOKENS - 1) / S::TOKENS;
     a.heads = 8;
     while (a.heads > 1 && token_blocks * ((a.H + a.heads - 1) / a.heads) < 2LL * cu_count()) a.heads /= 2;
     q_chunks = (a.H + a.heads - 1) / a.heads;
     q_blocks = token_blocks * q_chunks;
   }
   if (items + q_blocks > 0x7fffffffLL) return FA_ERR_DIMS;
-  return a.rot.interleaved ? launch_append_passes<E, D, true>(a, (int)q_blocks, q_chunks, touched, items + q_blocks)
-                           : launch_append_passes<E, D, false>(a, (int)q_blocks, q_chunks, touched, items + q_blocks);
+  hipLaunchKernelGGL((append_kernel<E, D, INTER, PASSES, NT>), dim3((unsigned)(items + q_blocks)), dim3(NT), 0,
+                     (hipStream_t)a.stream, a, (int)items, q_chunks, touched);
+  return hipGetLastError() == hipSuccess ? FA_OK : FA_ERR_LAUNCH;
+}
+
+template <typename E, int D>
+int launch_append(const AppendArgs& a) {
+  const int passes = std::max(1, a.cache.page_size / Slot<D>::TOKENS);
+#define FA_PASSES(P_, NT_) (a.rot.interleaved ? launch_append<E, D, true, P_, NT_>(a) : launch_append<E, D, false, P_, NT_>(a))
+  if (passes == 1) return FA_PASSES(1, 256);
+  if (passes == 2) return FA_PASSES(2, 256);
+  if constexpr (D >= 64) {
+    if (passes == 4) return FA_PASSES(4, 256);
+    if constexpr (D >= 128) return FA_PASSES(4, 512);
+  }
+#undef FA_PASSES
+  return FA_ERR_UNSUPPORTED;
 }
 
 // How a call's rows and keys are cut: blocks of `rows` rows, each block's keys in up to nsplit parts of

@@ -10,9 +10,10 @@
 // forward (fa_fwd.hip): S^T = K Q^T on 32x32x16 products with a lane owning one row, the scores fed
 // back as the B operand of O^T += V^T P^T, V^T read transposed from LDS, S(j + 1) under the softmax of
 // S(j).  What differs:
-//   * a 16-key part of a tile lies in one page: its K scale multiplies its scores, its V scale joins
+//   * a 16-key part of a tile (the whole tile with pages of 64 keys or more) lies in one page: its K scale multiplies its scores, its V scale joins
 //     their exponent, and leaves the row sums again, part by part;
-//   * pages and scales of 16 tiles at a time are kept one part to a lane and loaded a run ahead;
+//   * pages and scales of 16 tiles (64 with pages of 64 keys or more) at a time are kept one part to a lane
+//     and loaded a run ahead;
 //   * the diagonal starts at past_lens: tiles below it run without a mask; a value of V behind the last
 //     key is stored as zero, and a NaN in a masked tile is dealt with behind the loop (fa_paged.h).
 #include "fa_paged.h"
@@ -26,7 +27,8 @@ struct Flag {
 
 constexpr float kRowSumLimit = 32768.f;   // 2^kLazy: no p' passes fp16's range
 
-template <typename E, int D, int NW>
+// PPT: parts of a tile that may lie in different pages (1: pages of 64 keys or more; else 4, of 16 keys).
+template <typename E, int D, int NW, int PPT>
 __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void rows_kernel(PagedArgs a, int row_blocks) {
   constexpr int BM = 32 * NW, BN = kBlockKeys, NB = BN / 32, NT = 64 * NW;
@@ -38,6 +40,8 @@ void rows_kernel(PagedArgs a, int row_blocks) {
   constexpr int PCR = D / 16;                // 16-code pieces per row
   constexpr int PIECES = BN * PCR;
   constexpr int PT = (PIECES + NT - 1) / NT; // pieces per thread, K and V each
+  constexpr int RUN = 64 / PPT;              // tiles whose parts fill the lanes of a wave
+  constexpr int PART = BN / PPT;             // keys of a part
   const float NEG_INF = -__builtin_inff();
   // K buffers at [0, 2 TILE), V buffers at [2 TILE, 4 TILE)
   __shared__ __attribute__((aligned(1024))) unsigned char lds[4 * TILE];
@@ -84,8 +88,7 @@ void rows_kernel(PagedArgs a, int row_blocks) {
     for (int t = 0; t < KT; ++t) qf[t] = gload16(q + 16 * t);
   }
 
-  // ---- pages and scales: lane i holds those of part i (16 keys) of the run of 16 tiles from run0, and of
-  // the next run
+  // ---- pages and scales: lane i holds those of part i of the run of RUN tiles from run0, and of the next run
   struct Parts {
     uint32_t lo, hi;   // offset of its first row in the pools
     int ve;
@@ -93,11 +96,11 @@ void rows_kernel(PagedArgs a, int row_blocks) {
   };
   Parts cur{}, nxt{};
   auto part_page = [&](int t0) __attribute__((always_inline)) {   // of the run that starts at tile t0
-    const int key = first + t0 * BN + 16 * lane;
-    return key < last ? page_of(a.cache, b, key >> page_bits) : 0;
+    // (parts behind the last key: its page, so no other page's scale has a say)
+    return page_of(a.cache, b, min(first + t0 * BN + PART * lane, last - 1) >> page_bits);
   };
   auto part_place = [&](Parts& p, int t0, int page) __attribute__((always_inline)) {
-    const int key = first + t0 * BN + 16 * lane;
+    const int key = first + t0 * BN + PART * lane;
     const uint64_t at = ((((uint64_t)max(page, 0) * Hkv + hk) << page_bits) + (key & (ps - 1))) * D;
     p.lo = (uint32_t)at, p.hi = (uint32_t)(at >> 32);
   };
@@ -112,48 +115,42 @@ void rows_kernel(PagedArgs a, int row_blocks) {
   // ---- staging: piece i of this thread is 16 codes of row prow + i RP of a tile.  Rows i RP apart swizzle
   // alike, and the two 16-byte halves of a converted piece lie 16 bytes apart (one bit of the offset).
   constexpr int RP = NT / PCR;               // rows that the workgroup stages at once
-  const int prow = tid / PCR % BN;           // (D = 32: half the threads have a piece)
-  const int goff = prow % 16 * D + tid % PCR * 16;
+  const int prow = tid / PCR % BN;           // (D <= 64: some threads have no piece)
+  const uint32_t goff = prow % PART * D + tid % PCR * 16;
   const int kdst = prow * ROWB + (((tid % PCR * 2) ^ ((prow * CPR / 16) & (CPR - 1))) << 4);
   const int vdst = prow * ROWB + ((tid % PCR * 32) ^ ((32 * (prow & 3)) & (ROWB - 1)));
   const bool stages = PIECES >= NT || tid < PIECES;
   auto fetch = [&](const void* pool, int t, u32x4 (&w)[PT]) __attribute__((always_inline)) {
-    const uint32_t lo = t - run0 < 16 ? cur.lo : nxt.lo, hi = t - run0 < 16 ? cur.hi : nxt.hi;
-    // a piece's row lies in part prow / 16, the same for a whole wave (D = 32: for half a wave)
+    const bool now = t - run0 < RUN;
+    const uint32_t lo = now ? cur.lo : nxt.lo, hi = now ? cur.hi : nxt.hi;
     auto part = [&](int i) __attribute__((always_inline)) {
-      const int from = ((t - run0) & 15) * 4 + i;
+      const int from = ((t - run0) & (RUN - 1)) * PPT + i;
       const uint64_t at = (uint64_t)(uint32_t)__builtin_amdgcn_readlane(hi, from) << 32 |
                           (uint32_t)__builtin_amdgcn_readlane(lo, from);
       return static_cast<const uint8_t*>(pool) + at;
     };
 #pragma unroll
     for (int i = 0; i < PT; ++i) {
-      const uint8_t* p;
-      if constexpr (D == 32) {
-        const int i0 = wave * (64 / PCR) / 16 % (BN / 16);
-        p = lane < 32 ? part(i0) : part(i0 + 1);
+      // a piece's row lies in part row / PART, the same for a whole wave (16-key parts at D = 32: for half a wave)
+      if constexpr (PPT == 1) {
+        w[i] = *reinterpret_cast<const u32x4*>(part(0) + goff + i * RP * D);
+      } else if constexpr (D == 32) {
+        const int i0 = wave * (64 / PCR) / 16 % PPT;
+        const uint8_t* const p0 = part(i0);
+        const uint8_t* const p1 = part(i0 + 1);
+        w[i] = *reinterpret_cast<const u32x4*>((lane < 32 ? p0 : p1) + goff);
       } else {
-        p = part((wave * (64 / PCR) + i * RP) / 16);
+        w[i] = *reinterpret_cast<const u32x4*>(part((wave * (64 / PCR) % BN + i * RP) / 16) + goff);
       }
-      w[i] = *reinterpret_cast<const u32x4*>(p + goff);
-    }
-  };
-  // (a 16-byte write serves 8 lanes at a time over 128 bytes of banks: with every other four lanes' halves
-  // swapped those 8 pieces, 32 bytes apart, meet 8 different sixteenths)
-  const bool upper = (tid & 4) != 0;
-  const int half0 = upper ? 16 : 0;
-  auto put_as = [&](auto type, const u32x4 (&w)[PT], int dst, unsigned char* buf) __attribute__((always_inline)) {
-    typedef decltype(type) T;
-#pragma unroll
-    for (int i = 0; i < PT; ++i) {
-      const u32x4 x = upper ? u32x4{w[i][2], w[i][3], w[i][0], w[i][1]} : w[i];
-      lds_write16(buf, (dst ^ half0) + i * RP * ROWB, codes8<T>(x[0], x[1]));
-      lds_write16(buf, (dst ^ half0 ^ 16) + i * RP * ROWB, codes8<T>(x[2], x[3]));
     }
   };
   auto put_k = [&](const u32x4 (&w)[PT], unsigned char* buf) __attribute__((always_inline)) {
     if (!stages) return;
-    put_as(E{}, w, kdst, buf);
+#pragma unroll
+    for (int i = 0; i < PT; ++i) {
+      lds_write16(buf, kdst + i * RP * ROWB, codes8<E>(w[i][0], w[i][1]));
+      lds_write16(buf, (kdst ^ 16) + i * RP * ROWB, codes8<E>(w[i][2], w[i][3]));
+    }
   };
   auto put_v = [&](u32x4 (&w)[PT], int t, unsigned char* buf, auto full) __attribute__((always_inline)) {
     if (!stages) return;
@@ -170,7 +167,11 @@ void rows_kernel(PagedArgs a, int row_blocks) {
         if (any != 0) nan_met = 1;
       }
     }
-    put_as(F16{}, w, vdst, buf);
+#pragma unroll
+    for (int i = 0; i < PT; ++i) {
+      lds_write16(buf, vdst + i * RP * ROWB, codes8<F16>(w[i][0], w[i][1]));
+      lds_write16(buf, (vdst ^ 16) + i * RP * ROWB, codes8<F16>(w[i][2], w[i][3]));
+    }
   };
 
   // ---- per-lane LDS operand offsets (fa_fwd.hip)
@@ -212,18 +213,18 @@ void rows_kernel(PagedArgs a, int row_blocks) {
   };
   // scales of part i of tile t
   auto k_scale = [&](int t, int i) __attribute__((always_inline)) {
-    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(cur.ks), (t - run0) * 4 + i));
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(cur.ks), (t - run0) * PPT + i));
   };
   auto v_exp = [&](int t, int i) __attribute__((always_inline)) {
-    return __builtin_amdgcn_readlane(cur.ve, (t - run0) * 4 + i);
+    return __builtin_amdgcn_readlane(cur.ve, (t - run0) * PPT + i);
   };
   auto tile_max = [&](const f32x16 (&s)[NB], int t) __attribute__((always_inline)) {
     float top = NEG_INF;
 #pragma unroll
-    for (int i = 0; i < 2 * NB; ++i) {
-      float mx = s[i / 2][8 * (i & 1)];
+    for (int i = 0; i < PPT; ++i) {
+      float mx = NEG_INF;
 #pragma unroll
-      for (int g = 1; g < 8; ++g) mx = fmaxf(mx, s[i / 2][8 * (i & 1) + g]);
+      for (int g = 0; g < 32 / PPT; ++g) mx = fmaxf(mx, s[(32 / PPT * i + g) / 16][(32 / PPT * i + g) % 16]);
       top = fmaxf(top, __builtin_fmaf(mx, k_scale(t, i), (float)v_exp(t, i)));
     }
     return halfwave_max(top);
@@ -240,21 +241,27 @@ void rows_kernel(PagedArgs a, int row_blocks) {
   };
   // P^T of the tile against mrun; the row's sum of it (this lane's half), and in l that with the V scales
   // taken out.  Both in fp32 from p as it is: where scales lie far apart a key that counts may have a p' that
-  // fp16 rounds to nothing.
+  // fp16 rounds to nothing.  (On the matrix pipe, from P as rounded, the sums would also hang on the other rows
+  // of their column: its zeros hand on a NaN.)
   auto exp_tile = [&](const f32x16 (&s)[NB], int t, u32x4 (&pk)[2 * NB], float& l) __attribute__((always_inline)) {
     float sum = 0.f;
     l = 0.f;
 #pragma unroll
-    for (int i = 0; i < 2 * NB; ++i) {
-      const float ks = k_scale(t, i), off = (float)v_exp(t, i) - mrun;
-      float p[8];
+    for (int k = 0; k < PPT; ++k) {
+      const int ve = v_exp(t, k);
+      const float ks = k_scale(t, k), off = (float)ve - mrun;
+      float y = 0.f;
 #pragma unroll
-      for (int g = 0; g < 8; ++g) p[g] = fast_exp2(__builtin_fmaf(s[i / 2][8 * (i & 1) + g], ks, off));
+      for (int i = 2 * NB / PPT * k; i < 2 * NB / PPT * (k + 1); ++i) {
+        float p[8];
 #pragma unroll
-      for (int q = 0; q < 4; ++q) pk[i][q] = pack2<F16>(p[2 * q], p[2 * q + 1]);
-      const float y = ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+        for (int g = 0; g < 8; ++g) p[g] = fast_exp2(__builtin_fmaf(s[i / 2][8 * (i & 1) + g], ks, off));
+#pragma unroll
+        for (int q = 0; q < 4; ++q) pk[i][q] = pack2<F16>(p[2 * q], p[2 * q + 1]);
+        y += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+      }
       sum += y;
-      l = __builtin_fmaf(y, exp2i(-v_exp(t, i)), l);
+      l = __builtin_fmaf(y, exp2i(-ve), l);
     }
     return sum;
   };
@@ -331,11 +338,11 @@ void rows_kernel(PagedArgs a, int row_blocks) {
     };
     auto iteration = [&](int j, f32x16 (&sc)[NB], f32x16 (&sn)[NB], auto full) __attribute__((always_inline)) {
       // a run's pages are asked for at its predecessor's start, their scales half a run later
-      if ((j & 15) == 0) {
+      if (j % RUN == 0) {
         if (j > 0) cur = nxt, run0 = j;
-        nxt_page = part_page(j + 16);
-        part_place(nxt, j + 16, nxt_page);
-      } else if ((j & 15) == 8) {
+        nxt_page = part_page(j + RUN);
+        part_place(nxt, j + RUN, nxt_page);
+      } else if (j % RUN == RUN / 2) {
         part_scales(nxt, nxt_page);
       }
       __syncthreads();
@@ -353,7 +360,7 @@ void rows_kernel(PagedArgs a, int row_blocks) {
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) sa[nb] = sb[nb];
     }
-    if ((j & 15) == 0 && j > 0) cur = nxt, run0 = j;
+    if (j % RUN == 0 && j > 0) cur = nxt, run0 = j;
     __syncthreads();
     u32x4 pk[2 * NB];
     pv_pre(Vbuf(j));
@@ -429,8 +436,14 @@ template <typename E, int D>
 int launch_rows(const PagedArgs& a, int row_blocks, int block_rows) {
   const dim3 g((unsigned)((long long)a.B * a.cache.H_kv * row_blocks * a.nsplit)), t(2 * block_rows);
   hipStream_t st = (hipStream_t)a.stream;
-  if (block_rows == 128) hipLaunchKernelGGL((rows_kernel<E, D, 4>), g, t, 0, st, a, row_blocks);
-  else hipLaunchKernelGGL((rows_kernel<E, D, 8>), g, t, 0, st, a, row_blocks);
+  const bool whole = a.cache.page_size >= kBlockKeys;   // a tile in one page
+  if (block_rows == 128) {
+    if (whole) hipLaunchKernelGGL((rows_kernel<E, D, 4, 1>), g, t, 0, st, a, row_blocks);
+    else hipLaunchKernelGGL((rows_kernel<E, D, 4, 4>), g, t, 0, st, a, row_blocks);
+  } else {
+    if (whole) hipLaunchKernelGGL((rows_kernel<E, D, 8, 1>), g, t, 0, st, a, row_blocks);
+    else hipLaunchKernelGGL((rows_kernel<E, D, 8, 4>), g, t, 0, st, a, row_blocks);
+  }
   return hipGetLastError() == hipSuccess ? FA_OK : FA_ERR_LAUNCH;
 }
 

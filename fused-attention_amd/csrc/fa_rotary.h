@@ -62,6 +62,10 @@ struct Turn {
     return a.positions_int64 ? static_cast<const long long*>(a.positions)[at] : static_cast<const int*>(a.positions)[at];
   }
 
+  __device__ __forceinline__ static int axis_of(const RotaryArgs& a, int pair) {
+    return (a.axes > 1 && pair >= a.section_end[0] ? 1 : 0) + (a.axes > 2 && pair >= a.section_end[1] ? 1 : 0);
+  }
+
   // Factors of token (b, n) for dims d0 .. d0 + 7.  A negative position leaves the row unturned
   // (padding); one past the table gives NaN.
   __device__ __forceinline__ void load(const RotaryArgs& a, int lane, int d0, int b, int n, long long base) {
@@ -76,8 +80,9 @@ struct Turn {
     constexpr int NP = INTER ? 4 : 8;   // pairs of this lane
     const int pair0 = INTER ? d0 / 2 : (d0 < half ? d0 : d0 - half);
     float cc[NP], ss[NP];
-    if (a.axes == 1) {
-      const long long p = position(a, 0, b, n, base);
+    const int axis = axis_of(a, pair0);
+    const long long p = position(a, axis, b, n, base);
+    if (axis == axis_of(a, pair0 + NP - 1)) {
       const float* row = a.table + (p < 0 ? 0 : p >= a.table_len ? 0 : p) * a.rotary_dim + pair0;
 #pragma unroll
       for (int i = 0; i < NP; i += 4) {
@@ -92,23 +97,26 @@ struct Turn {
         ss[i] = p < 0 ? 0.f : ss[i] + bad;
       }
     } else {
-      // (every axis' position, then every table value: two waits, not two a pair)
-      const long long p0 = position(a, 0, b, n, base), p1 = position(a, 1, b, n, base);
-      const long long p2 = a.axes > 2 ? position(a, 2, b, n, base) : p1;
-      const int end0 = a.section_end[0], end1 = a.axes > 2 ? a.section_end[1] : half;
-      long long p[NP];
+      // a section ends among this lane's pairs: every axis' position, then every table value
+      long long q[kMaxAxes];
 #pragma unroll
-      for (int i = 0; i < NP; ++i) p[i] = pair0 + i < end0 ? p0 : pair0 + i < end1 ? p1 : p2;
+      for (int i = 0; i < kMaxAxes; ++i) q[i] = position(a, min(i, a.axes - 1), b, n, base);
+      long long at[NP];
 #pragma unroll
       for (int i = 0; i < NP; ++i) {
-        const float* row = a.table + (p[i] >= 0 && p[i] < a.table_len ? p[i] : 0) * a.rotary_dim + pair0 + i;
+        const int k = axis_of(a, pair0 + i);
+        at[i] = k == 0 ? q[0] : k == 1 ? q[1] : q[2];
+      }
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+        const float* row = a.table + (at[i] >= 0 && at[i] < a.table_len ? at[i] : 0) * a.rotary_dim + pair0 + i;
         cc[i] = row[0], ss[i] = row[half];
       }
 #pragma unroll
       for (int i = 0; i < NP; ++i) {
-        const float bad = p[i] >= a.table_len ? __builtin_nanf("") : 0.f;
-        cc[i] = p[i] < 0 ? 1.f : cc[i] + bad;
-        ss[i] = p[i] < 0 ? 0.f : ss[i] + bad;
+        const float bad = at[i] >= a.table_len ? __builtin_nanf("") : 0.f;
+        cc[i] = at[i] < 0 ? 1.f : cc[i] + bad;
+        ss[i] = at[i] < 0 ? 0.f : ss[i] + bad;
       }
     }
     if constexpr (INTER) {
@@ -166,16 +174,17 @@ __device__ __forceinline__ float inv_rms(const float (&x)[8], float eps) {
   return 1.0f / __builtin_sqrtf(team_sum<D / 8>(ss) * (1.0f / D) + eps);
 }
 
-// One row: x packed (and its partner's), cw = C w and sw = S w_partner of its token and tensor.
+// One row: x packed (and its partner's), cw = C w and sw = S w_partner of its token and tensor.  The row is
+// z times the value returned.
 template <typename E, int D, bool INTER>
-__device__ __forceinline__ void turn_row(const u32x4& w, const u32x4& wp, const float (&cw)[8], const float (&sw)[8],
-                                         bool norm, float eps, float (&y)[8]) {
+__device__ __forceinline__ float turn_row(const u32x4& w, const u32x4& wp, const float (&cw)[8], const float (&sw)[8],
+                                          bool norm, float eps, float (&z)[8]) {
   float x[8], xp[8];
   unpack8<E>(w, x);
   unpack8<E>(wp, xp);
-  const float r = norm ? inv_rms<D>(x, eps) : 1.f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) y[i] = r * __builtin_fmaf(x[i], cw[i], partner_of<INTER>(xp, i) * sw[i]);
+  for (int i = 0; i < 8; ++i) z[i] = __builtin_fmaf(x[i], cw[i], partner_of<INTER>(xp, i) * sw[i]);
+  return norm ? inv_rms<D>(x, eps) : 1.f;
 }
 
 // The weights of a lane's dims and of their partners (in place of the partners' own order when
@@ -201,10 +210,10 @@ __device__ __forceinline__ void fold_weights(const Turn<D, INTER>& t, const floa
 constexpr int kRowThreads = 256;
 constexpr int kRowBatch = 4;     // heads whose rows are in flight at a time
 
-template <int D>
+template <int D, int NT = kRowThreads>
 struct Slot {
-  static constexpr int TPR = D / 8;                 // lanes per row
-  static constexpr int TOKENS = kRowThreads / TPR;  // rows a workgroup holds at once
+  static constexpr int TPR = D / 8;        // lanes per row
+  static constexpr int TOKENS = NT / TPR;  // rows a workgroup of NT threads holds at once
 };
 
 // Heads h0 .. h1 - 1 of token (b, n): one team of lanes, the heads one after another, the token's
@@ -227,7 +236,9 @@ __device__ __forceinline__ void turn_heads(const RotaryArgs& rot, const void* w,
 #pragma unroll
     for (int i = 0; i < kRowBatch; ++i) {
       float y[8];
-      turn_row<E, D, INTER>(x[i], turn.fetch(x[i]), cw, sw, w != nullptr, rot.eps, y);
+      const float r = turn_row<E, D, INTER>(x[i], turn.fetch(x[i]), cw, sw, w != nullptr, rot.eps, y);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) y[j] *= r;
       if (valid && h + i < h1) gstore16(dst + (h + i) * out.stride_h, pack8<E>(y));
     }
   }
