@@ -150,6 +150,9 @@ inline int occupancy_per_cu(const void* kern, int threads) {
   return per_cu;
 }
 
+// Whether a launch's threads stay below the runtime's 2^32.
+inline bool grid_fits(long long workgroups, int threads) { return workgroups <= 0xffffffffLL / threads; }
+
 #define set_smem_once(kern, SMEM)                                   \
   ([&]() {                                                          \
     static const bool ok_ = ::fa::smem_attr<SMEM>(kern);            \

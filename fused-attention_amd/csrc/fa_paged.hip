@@ -586,7 +586,7 @@ int launch_append(AppendArgs a) {
     q_chunks = (a.H + a.heads - 1) / a.heads;
     q_blocks = token_blocks * q_chunks;
   }
-  if (items + q_blocks > 0x7fffffffLL) return FA_ERR_DIMS;
+  if (!grid_fits(items + q_blocks, NT)) return FA_ERR_DIMS;
   hipLaunchKernelGGL((append_kernel<E, D, INTER, PASSES, NT>), dim3((unsigned)(items + q_blocks)), dim3(NT), 0,
                      (hipStream_t)a.stream, a, (int)items, q_chunks, touched);
   return hipGetLastError() == hipSuccess ? FA_OK : FA_ERR_LAUNCH;
@@ -656,7 +656,8 @@ template <typename E, int D>
 int launch_attend(const PagedArgs& a, const Cut& c, int dtype) {
   const long long grid = (long long)a.B * a.cache.H_kv * c.row_blocks * a.nsplit;
   const long long joins = (long long)a.B * a.H * a.N;
-  if (grid > 0x7fffffffLL || joins > 0x7fffffffLL) return FA_ERR_DIMS;
+  if (!grid_fits(grid, c.rows == kRows ? 64 * kWaves : 2 * c.rows)) return FA_ERR_DIMS;
+  if (a.nsplit > kFewSplits && !grid_fits(joins, kJoinThreads)) return FA_ERR_DIMS;
   hipStream_t st = (hipStream_t)a.stream;
   if (c.rows == kRows) {
     hipLaunchKernelGGL((attend_kernel<E, D>), dim3((unsigned)grid), dim3(64 * kWaves), 0, st, a, c.row_blocks);

@@ -195,13 +195,13 @@ void rows_kernel(PagedArgs a, int row_blocks) {
   float lsum = 0.f;   // of this lane's half of the keys
 
   auto s_tile = [&](const unsigned char* Ks, f32x16 (&s)[NB]) __attribute__((always_inline)) {
+    f32x16 y[NB] = {};
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
-      f32x16 y = f32x16{};
+    for (int t = 0; t < KT; ++t)
 #pragma unroll
-      for (int t = 0; t < KT; ++t) y = mfma32<E>(lds_read16(Ks, koff[t] + nb * 32 * ROWB), qf[t], y);
-      s[nb] = y;
-    }
+      for (int nb = 0; nb < NB; ++nb) y[nb] = mfma32<E>(lds_read16(Ks, koff[t] + nb * 32 * ROWB), qf[t], y[nb]);
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) s[nb] = y[nb];
   };
   auto mask_tile = [&](f32x16 (&s)[NB], int k0) __attribute__((always_inline)) {
     const int t = lim - k0 - 4 * hh;

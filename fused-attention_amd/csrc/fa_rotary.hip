@@ -167,7 +167,7 @@ int launch_qk(QkArgs a, bool bwd) {
   a.heads = p.heads;
   a.blocks = bwd_blocks(p);
   const long long grid = bwd ? (long long)a.blocks * p.chunks : p.token_blocks * p.chunks;
-  if (grid > 0x7fffffffLL) return FA_ERR_DIMS;
+  if (!grid_fits(grid, kRowThreads)) return FA_ERR_DIMS;
   const dim3 g((unsigned)grid), t(kRowThreads);
   hipStream_t st = (hipStream_t)a.stream;
   if (bwd) {
