@@ -42,8 +42,10 @@ __device__ __forceinline__ void decode8(const u32x2& w, float (&y)[8]) {
 // nobody else writes its codes and scale: it holds the page's new rows in registers, reduces their largest
 // value, and writes codes.  The others turn the queries (turn_heads); the pages, whose chain of waits is
 // longer, go first (queries first: +3 % at B=2 H=32 H_kv=8 N=8192 D=128, +5 % at N=1).  PASSES: rows of a page
-// over the rows that the workgroup holds at once; four at most, or the registers leave too few waves (128-row
-// pages at D = 128: eight passes of 256 threads 101 us, four of 512 95; 64-row pages: four of 256 90, two of 512 91).
+// over the rows that the workgroup's NT threads hold at once; four at most, or the registers leave too few waves
+// (128-row pages at D = 128: eight passes of 256 threads 101 us, four of 512 95; 64-row pages: four of 256 90, two
+// of 512 91), and no more threads than a page has pieces (16-row pages at D = 64, B=3 N=1000: 256 threads 9.3 us,
+// 128 7.1).
 template <typename E, int D, bool INTER, int PASSES, int NT>
 __global__ __launch_bounds__(NT) void append_kernel(AppendArgs a, int items, int q_chunks, int touched) {
   using S = Slot<D, NT>;
@@ -594,13 +596,14 @@ int launch_append(AppendArgs a) {
 
 template <typename E, int D>
 int launch_append(const AppendArgs& a) {
-  const int passes = std::max(1, a.cache.page_size / Slot<D>::TOKENS);
 #define FA_PASSES(P_, NT_) (a.rot.interleaved ? launch_append<E, D, true, P_, NT_>(a) : launch_append<E, D, false, P_, NT_>(a))
-  if (passes == 1) return FA_PASSES(1, 256);
-  if (passes == 2) return FA_PASSES(2, 256);
-  if constexpr (D >= 64) {
-    if (passes == 4) return FA_PASSES(4, 256);
-    if constexpr (D >= 128) return FA_PASSES(4, 512);
+  switch (a.cache.page_size * Slot<D>::TPR) {   // threads for a page's rows at once
+    case 64: return FA_PASSES(1, 64);
+    case 128: return FA_PASSES(1, 128);
+    case 256: return FA_PASSES(1, 256);
+    case 512: return FA_PASSES(2, 256);
+    case 1024: return FA_PASSES(4, 256);
+    case 2048: return FA_PASSES(4, 512);
   }
 #undef FA_PASSES
   return FA_ERR_UNSUPPORTED;
