@@ -172,8 +172,8 @@ __global__ __launch_bounds__(NT) void append_kernel(AppendArgs a, int items, int
 // ---------------------------------------------------------------------------
 // Attention of few rows (the mathematics: fa_paged.h).
 //
-// Rows: the N x G queries of a K/V head (G = H / H_kv), row r = token r / G, head r % G: 16 to a
-// workgroup, so each key's bytes serve all of them.  S^T = K Q^T as 16x16x32 products (16 keys x 16
+// Rows: the N x G queries of a K/V head (G = H / H_kv), row r = token r / G, head r % G: 16, 32 or 64
+// to a workgroup, so each key's bytes serve all of them.  S^T = K Q^T as 16x16x32 products (16 keys x 16
 // rows): a lane owns one row, and the scores are fed back as the B operand of O^T += V^T P^T.  Two
 // 16-key tiles fill its 32 contraction slots; with slot (group g, j) = key 16 (j / 4) + 4 g + j % 4
 // no score moves between lanes, and V is read in that order, straight from the pages' rows: a lane
@@ -235,15 +235,17 @@ struct Tile {
   }
 };
 
-template <typename E, int D>
-__global__ __launch_bounds__(64 * kWaves) void attend_kernel(PagedArgs a, int row_blocks) {
+// RT: 16-row blocks that a wave holds; each converted K and V operand serves all of them.
+template <typename E, int D, int RT>
+__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(RT <= 2 ? 2 : 1))) void attend_kernel(PagedArgs a, int row_blocks) {
   typedef Tile<D> T;
   constexpr int VB = T::VB;
   constexpr int KT = D / 32;         // contraction steps over D
   constexpr int LD = D + 4;          // row of the merge buffer
+  constexpr int BR = kRows * RT;     // rows of the workgroup
   const float NEG_INF = -__builtin_inff();
-  __shared__ __attribute__((aligned(16))) float merge[kWaves][kRows][LD];
-  __shared__ float ml[kWaves][2][kRows];
+  __shared__ __attribute__((aligned(16))) float merge[kWaves][BR][LD];
+  __shared__ float ml[kWaves][2][BR];
 
   const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -252,27 +254,28 @@ __global__ __launch_bounds__(64 * kWaves) void attend_kernel(PagedArgs a, int ro
   const long long block = blockIdx.x / a.nsplit;
   const int rb = block % row_blocks, bh = block / row_blocks;
   const int b = bh / Hkv, hk = bh % Hkv;
-  const Block x = block_of(a, b, rb, G, kRows);
+  const Block x = block_of(a, b, rb, G, BR);
   const int per = split_keys(x.keys, a.nsplit, kSplitStep);
   const int first = split * per, last = min(first + per, x.keys);   // keys of this workgroup
   if (split > 0 && first >= x.keys) return;                        // (the first split also writes what has no keys)
 
-  const int r = min(x.r0 + c, x.rows - 1), tok = r / G, head = hk * G + r % G;
-  const int lim = x.r0 + c < x.rows && tok < x.fresh ? x.past + tok : -1;    // last key this lane's row sees
-
-  // Q^T: column c, dims of step s: 64 (s / 2) + 16 g + 8 (s % 2) (D = 32: 8 g)
+  // Q^T: column c of each block, dims of step s: 64 (s / 2) + 16 g + 8 (s % 2) (D = 32: 8 g)
   auto dim_of = [&](int s) __attribute__((always_inline)) { return D == 32 ? 8 * g : 64 * (s >> 1) + 16 * g + 8 * (s & 1); };
-  u32x4 qf[KT];
-  {
+  u32x4 qf[RT][KT];
+  int lim[RT];    // last key that this lane's rows see
+  f32x4 acc[RT][VB];
+  float m[RT], l[RT];
+#pragma unroll
+  for (int t = 0; t < RT; ++t) {
+    const int at = x.r0 + 16 * t + c, r = min(at, x.rows - 1), tok = r / G, head = hk * G + r % G;
+    lim[t] = at < x.rows && tok < x.fresh ? x.past + tok : -1;
     const uint16_t* q = static_cast<const uint16_t*>(a.q.data) + b * a.q.stride_b + head * a.q.stride_h + tok * a.q.stride_n;
 #pragma unroll
-    for (int s = 0; s < KT; ++s) qf[s] = gload16(q + dim_of(s));
-  }
-
-  f32x4 acc[VB];
+    for (int s = 0; s < KT; ++s) qf[t][s] = gload16(q + dim_of(s));
 #pragma unroll
-  for (int i = 0; i < VB; ++i) acc[i] = f32x4{};
-  float m = -__FLT_MAX__, l = 0.f;
+    for (int i = 0; i < VB; ++i) acc[t][i] = f32x4{};
+    m[t] = -__FLT_MAX__, l[t] = 0.f;
+  }
   const uint8_t* const kp = static_cast<const uint8_t*>(a.cache.k);
   const uint8_t* const vp = static_cast<const uint8_t*>(a.cache.v);
 
@@ -310,17 +313,24 @@ __global__ __launch_bounds__(64 * kWaves) void attend_kernel(PagedArgs a, int ro
   bool nan_met = false;   // a masked step of V held a NaN
 
   auto compute = [&](T (&t)[2], int i, int k0) __attribute__((always_inline)) {
-    f32x4 s[2];
+    f32x4 s[RT][2];
     int ve[2];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const float ks = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(my_ks), i + u));
       ve[u] = __builtin_amdgcn_readlane(my_ve, i + u);
-      s[u] = f32x4{};
 #pragma unroll
-      for (int n = 0; n < KT; ++n) s[u] = mfma16<E>(codes8<E>(t[u].k[2 * n], t[u].k[2 * n + 1]), qf[n], s[u]);
+      for (int r = 0; r < RT; ++r) s[r][u] = f32x4{};
 #pragma unroll
-      for (int n = 0; n < 4; ++n) s[u][n] = __builtin_fmaf(s[u][n], ks, (float)ve[u]);
+      for (int n = 0; n < KT; ++n) {
+        const u32x4 k = codes8<E>(t[u].k[2 * n], t[u].k[2 * n + 1]);
+#pragma unroll
+        for (int r = 0; r < RT; ++r) s[r][u] = mfma16<E>(k, qf[r][n], s[r][u]);
+      }
+#pragma unroll
+      for (int r = 0; r < RT; ++r)
+#pragma unroll
+        for (int n = 0; n < 4; ++n) s[r][u][n] = __builtin_fmaf(s[r][u][n], ks, (float)ve[u]);
     }
     if (k0 + kStep - 1 > x.lmin) {
 #pragma unroll
@@ -328,7 +338,9 @@ __global__ __launch_bounds__(64 * kWaves) void attend_kernel(PagedArgs a, int ro
 #pragma unroll
         for (int n = 0; n < 4; ++n) {
           const int key = k0 + 16 * u + 4 * g + n;
-          if (key > lim) s[u][n] = NEG_INF;
+#pragma unroll
+          for (int r = 0; r < RT; ++r)
+            if (key > lim[r]) s[r][u][n] = NEG_INF;
 #pragma unroll
           for (int w = 0; w < T::VW; ++w) {   // what lies behind the last key may be anything
             const uint32_t v = key >= x.keys ? 0u : t[u].v[n][w], nan = nan_bytes(v);
@@ -337,28 +349,36 @@ __global__ __launch_bounds__(64 * kWaves) void attend_kernel(PagedArgs a, int ro
           }
         }
     }
-    float mx = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
-                     fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
-    mx = groups_max(mx);
-    if (__builtin_amdgcn_ballot_w64(mx > m + kLazy)) {
-      const float mn = mx > m + kLazy ? mx - kBelow : m;   // (a row's own scores alone move it)
-      const float alpha = fast_exp2(m - mn);
-      m = mn;
-      l *= alpha;
+    u32x4 pf[RT];
 #pragma unroll
-      for (int n = 0; n < VB; ++n) acc[n] *= alpha;
+    for (int r = 0; r < RT; ++r) {
+      float mx = fmaxf(fmaxf(fmaxf(s[r][0][0], s[r][0][1]), fmaxf(s[r][0][2], s[r][0][3])),
+                       fmaxf(fmaxf(s[r][1][0], s[r][1][1]), fmaxf(s[r][1][2], s[r][1][3])));
+      mx = groups_max(mx);
+      if (__builtin_amdgcn_ballot_w64(mx > m[r] + kLazy)) {
+        const float mn = mx > m[r] + kLazy ? mx - kBelow : m[r];   // (a row's own scores alone move it)
+        const float alpha = fast_exp2(m[r] - mn);
+        m[r] = mn;
+        l[r] *= alpha;
+#pragma unroll
+        for (int n = 0; n < VB; ++n) acc[r][n] *= alpha;
+      }
+      float p[2][4];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+#pragma unroll
+        for (int n = 0; n < 4; ++n) p[u][n] = fast_exp2(s[r][u][n] - m[r]);
+        l[r] = __builtin_fmaf((p[u][0] + p[u][1]) + (p[u][2] + p[u][3]), exp2i(-ve[u]), l[r]);
+      }
+      pf[r] = u32x4{pack2<F16>(p[0][0], p[0][1]), pack2<F16>(p[0][2], p[0][3]), pack2<F16>(p[1][0], p[1][1]),
+                    pack2<F16>(p[1][2], p[1][3])};
     }
-    float p[2][4];
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
+    for (int y = 0; y < VB; ++y) {
+      const u32x4 v = v_operand(t, y);
 #pragma unroll
-      for (int n = 0; n < 4; ++n) p[u][n] = fast_exp2(s[u][n] - m);
-      l = __builtin_fmaf((p[u][0] + p[u][1]) + (p[u][2] + p[u][3]), exp2i(-ve[u]), l);
+      for (int r = 0; r < RT; ++r) acc[r][y] = mfma16<F16>(v, pf[r], acc[r][y]);
     }
-    const u32x4 pf = {pack2<F16>(p[0][0], p[0][1]), pack2<F16>(p[0][2], p[0][3]), pack2<F16>(p[1][0], p[1][1]),
-                      pack2<F16>(p[1][2], p[1][3])};
-#pragma unroll
-    for (int y = 0; y < VB; ++y) acc[y] = mfma16<F16>(v_operand(t, y), pf, acc[y]);
   };
 
   // The next step's bytes are on their way while a step is computed; past the last one its own
@@ -382,7 +402,7 @@ __global__ __launch_bounds__(64 * kWaves) void attend_kernel(PagedArgs a, int ro
       const int k0 = first + (j * kWaves + wave) * kStep;
       if (k0 + kStep - 1 <= x.lmin || k0 >= last) continue;
       T t[2];
-      u32x4 seen;
+      u32x4 seen[RT];
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         const int key = k0 + 16 * u;
@@ -394,61 +414,71 @@ __global__ __launch_bounds__(64 * kWaves) void attend_kernel(PagedArgs a, int ro
           for (int w = 0; w < T::VW; ++w) t[u].v[n][w] = key + 4 * g + n < x.keys ? nan_as_one(t[u].v[n][w]) : 0u;
 #pragma unroll
         for (int n = 0; n < 2; ++n)
-          seen[2 * u + n] = (key + 4 * g + 2 * n <= lim ? 0x3C00u : 0u) | (key + 4 * g + 2 * n + 1 <= lim ? 0x3C000000u : 0u);
+#pragma unroll
+          for (int r = 0; r < RT; ++r)
+            seen[r][2 * u + n] = (key + 4 * g + 2 * n <= lim[r] ? 0x3C00u : 0u) | (key + 4 * g + 2 * n + 1 <= lim[r] ? 0x3C000000u : 0u);
       }
 #pragma unroll
-      for (int y = 0; y < VB; ++y) {
-        const f32x4 count = mfma16<F16>(v_operand(t, y), seen, f32x4{});
+      for (int y = 0; y < VB; ++y)
 #pragma unroll
-        for (int n = 0; n < 4; ++n)
-          if (count[n] > 0.f) acc[y][n] = __builtin_nanf("");
-      }
+        for (int r = 0; r < RT; ++r) {
+          const f32x4 count = mfma16<F16>(v_operand(t, y), seen[r], f32x4{});
+#pragma unroll
+          for (int n = 0; n < 4; ++n)
+            if (count[n] > 0.f) acc[r][y][n] = __builtin_nanf("");
+        }
     }
   }
 
   // merge of the waves: lane (c, g) holds row c, dims 4 g VB .. + 4 VB - 1
-  l = groups_sum(l);
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int r = 0; r < RT; ++r) {
+    const float sum = groups_sum(l[r]);
 #pragma unroll
-    for (int y = 0; y < VB; ++y) merge[wave][c][(4 * g + i) * VB + y] = acc[y][i];
-  if (g == 0) ml[wave][0][c] = m, ml[wave][1][c] = l;
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int y = 0; y < VB; ++y) merge[wave][16 * r + c][(4 * g + i) * VB + y] = acc[r][y][i];
+    if (g == 0) ml[wave][0][16 * r + c] = m[r], ml[wave][1][16 * r + c] = sum;
+  }
   __syncthreads();
   constexpr int PER = kRows * D / (64 * kWaves);   // values per thread (D = 32: 2)
   constexpr int TR = D / PER;                      // threads per row
-  const int row = threadIdx.x / TR, d0 = threadIdx.x % TR * PER;
-  const int rr = x.r0 + row;
-  if (rr >= x.rows) return;
-  const int ot = rr / G, oh = hk * G + rr % G;
-  float M = -__FLT_MAX__, f[kWaves], L = 0.f, o[PER];
+  const int d0 = threadIdx.x % TR * PER;
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) M = fmaxf(M, ml[w][0][row]);
+  for (int t = 0; t < RT; ++t) {
+    const int row = 16 * t + threadIdx.x / TR, rr = x.r0 + row;
+    if (rr >= x.rows) return;
+    const int ot = rr / G, oh = hk * G + rr % G;
+    float M = -__FLT_MAX__, f[kWaves], L = 0.f, o[PER];
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) {
-    f[w] = fast_exp2(ml[w][0][row] - M);
-    L = __builtin_fmaf(f[w], ml[w][1][row], L);
+    for (int w = 0; w < kWaves; ++w) M = fmaxf(M, ml[w][0][row]);
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      f[w] = fast_exp2(ml[w][0][row] - M);
+      L = __builtin_fmaf(f[w], ml[w][1][row], L);
+    }
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      float z = 0.f;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) z = __builtin_fmaf(f[w], merge[w][row][d0 + i], z);
+      o[i] = z;
+    }
+    if (per < x.keys) {   // more than one split: the join divides
+      float* const dst = part_row<D>(a, block, split, row, BR);
+#pragma unroll
+      for (int i = 0; i < PER; ++i) dst[d0 + i] = o[i];
+      if (d0 == 0) dst[D] = M, dst[D + 1] = L;
+      continue;
+    }
+    const bool live = ot < x.fresh;
+    const float inv = live ? 1.0f / L : 0.f;
+    uint16_t* dst = static_cast<uint16_t*>(const_cast<void*>(a.o.data)) + b * a.o.stride_b + oh * a.o.stride_h + ot * a.o.stride_n + d0;
+#pragma unroll
+    for (int i = 0; i < PER; i += 2)
+      *reinterpret_cast<uint32_t*>(dst + i) = live ? pack2<E>(o[i] * inv, o[i + 1] * inv) : 0u;
+    if (a.lse != nullptr && d0 == 0) a.lse[((long long)b * a.H + oh) * a.N + ot] = live ? M + __log2f(L) : NEG_INF;
   }
-#pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    float z = 0.f;
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) z = __builtin_fmaf(f[w], merge[w][row][d0 + i], z);
-    o[i] = z;
-  }
-  if (per < x.keys) {   // more than one split: the join divides
-    float* const dst = part_row<D>(a, block, split, row, kRows);
-#pragma unroll
-    for (int i = 0; i < PER; ++i) dst[d0 + i] = o[i];
-    if (d0 == 0) dst[D] = M, dst[D + 1] = L;
-    return;
-  }
-  const bool live = ot < x.fresh;
-  const float inv = live ? 1.0f / L : 0.f;
-  uint16_t* dst = static_cast<uint16_t*>(const_cast<void*>(a.o.data)) + b * a.o.stride_b + oh * a.o.stride_h + ot * a.o.stride_n + d0;
-#pragma unroll
-  for (int i = 0; i < PER; i += 2)
-    *reinterpret_cast<uint32_t*>(dst + i) = live ? pack2<E>(o[i] * inv, o[i + 1] * inv) : 0u;
-  if (a.lse != nullptr && d0 == 0) a.lse[((long long)b * a.H + oh) * a.N + ot] = live ? M + __log2f(L) : NEG_INF;
 }
 
 // Joins the splits of a row, a workgroup to a row: D / 4 threads a split, 1024 / D splits at a time.
@@ -620,17 +650,22 @@ struct Cut {
 // and more partial rows: us at 1 / 2 / 4 workgroups to a CU, 8 sequences of 1335 to 4005 keys, 8 K/V heads, D = 128:
 // 17.4 / 20.7 / 26.4; 64 of 667 to 2000 keys 36.1 / 36.2 / 40.8; one of 16000 keys 13.8 / 15.5 / 24.9), up to
 // four where a part keeps 4096 keys, for lengths that differ (32 sequences of 5461 to 16384 keys 140.9 / 141.9 / 135.3).
-// Many rows: 32 rows go to the kernel of few rows, 128 to 128-row workgroups, more to 256-row ones (us of 16 /
-// 128 / 256 rows; 8 sequences of 4000 keys, 8 K/V heads, D = 128: 32 rows 28 / 32 / 40, 64 rows 38 / 35 / 42, 128 rows
-// 59 / 40 / 46, 256 rows 96 / 60 / 58, 512 rows 199 / 93 / 91), and the parts are those of the least cost by the
-// times that a tile of one workgroup to a CU, a workgroup's start and the join of its partial rows take.
+// Up to 64 rows go to the kernel of few rows, in one block of 16, 32 or 64 (us of blocks of 16 / 32 / 64 / 128-row
+// workgroups; 8 sequences of 4000 keys, 8 K/V heads, D = 128: 32 rows 28 / 21 / - / 32, 64 rows 38 / - / 28 / 34), but
+// in two of 16 where the parts of one would not reach all CUs (one K/V head, 16384 keys, D = 64, 32 rows: 8.7 against
+// 9.6 in one block); 128 rows to 128-row workgroups, more to 256-row ones (us of 128 / 256 rows: 128 rows 40 / 46, 256
+// rows 60 / 58, 512 rows 93 / 91).  Their parts are those of the least cost by the times that a tile of one
+// workgroup to a CU, a workgroup's start and the join of its partial rows take.
 Cut cut_of(int B, int H, int Hkv, int N, int D, long long keys) {
   Cut c;
   const long long rows = (long long)N * (H / Hkv), units = (long long)B * Hkv;
-  c.rows = rows <= 32 ? kRows : rows <= 128 ? 128 : 256;
+  const long long cus = cu_count();
+  c.rows = 16;
+  while (c.rows < rows && c.rows < 256) c.rows *= 2;
+  if (c.rows == 32 && units * (keys / kSplitStep) < cus) c.rows = 16;
   c.row_blocks = (int)((rows + c.rows - 1) / c.rows);
-  const long long blocks = units * c.row_blocks, cus = cu_count();
-  if (c.rows == kRows) {
+  const long long blocks = units * c.row_blocks;
+  if (c.rows <= 64) {
     c.step = kSplitStep;
     const long long fill = (cus + blocks - 1) / blocks, four = (4 * cus + blocks - 1) / blocks;
     c.nsplit = (int)std::max<long long>(1, std::min<long long>({std::max(fill, std::min(four, keys / 4096)),
@@ -659,11 +694,15 @@ template <typename E, int D>
 int launch_attend(const PagedArgs& a, const Cut& c, int dtype) {
   const long long grid = (long long)a.B * a.cache.H_kv * c.row_blocks * a.nsplit;
   const long long joins = (long long)a.B * a.H * a.N;
-  if (!grid_fits(grid, c.rows == kRows ? 64 * kWaves : 2 * c.rows)) return FA_ERR_DIMS;
+  if (!grid_fits(grid, c.rows <= 64 ? 64 * kWaves : 2 * c.rows)) return FA_ERR_DIMS;
   if (a.nsplit > kFewSplits && !grid_fits(joins, kJoinThreads)) return FA_ERR_DIMS;
   hipStream_t st = (hipStream_t)a.stream;
-  if (c.rows == kRows) {
-    hipLaunchKernelGGL((attend_kernel<E, D>), dim3((unsigned)grid), dim3(64 * kWaves), 0, st, a, c.row_blocks);
+  if (c.rows == 16) {
+    hipLaunchKernelGGL((attend_kernel<E, D, 1>), dim3((unsigned)grid), dim3(64 * kWaves), 0, st, a, c.row_blocks);
+  } else if (c.rows == 32) {
+    hipLaunchKernelGGL((attend_kernel<E, D, 2>), dim3((unsigned)grid), dim3(64 * kWaves), 0, st, a, c.row_blocks);
+  } else if (c.rows == 64) {
+    hipLaunchKernelGGL((attend_kernel<E, D, 4>), dim3((unsigned)grid), dim3(64 * kWaves), 0, st, a, c.row_blocks);
   } else {
     const int status = paged_rows(dtype, a, c.row_blocks, c.rows);
     if (status != FA_OK) return status;

@@ -103,13 +103,13 @@ def test_attention_heads_and_rows(H, Hkv, N):
 def test_attention_lengths(total):
     cache = filled(100, 1, 16, 128, total, spread=3)
     bt = tables(1, 100, 100, total)
-    for N in (1, 3, 40):
+    for N in (1, 3, 7, 13, 25, 70):   # 4 to 280 rows: every size of row block
         if N <= total:
             q = randn(total + N, 1, 4, N, 128).to(torch.float16)
             check_attend(q, cache, bt, ints(total - N), label=f"total={total} N={N}")
 
 
-@pytest.mark.parametrize("N", [4, 100])
+@pytest.mark.parametrize("N", [4, 9, 18, 100])
 def test_padded_batch_and_empty_sequences(N):
     cache = filled(64, 2, 16, 64, 1, spread=2)
     bt = tables(4, 16, 64, 2)
@@ -122,7 +122,7 @@ def test_padded_batch_and_empty_sequences(N):
     assert torch.equal(a, fused_paged_attention(q, cache, bt, ints(7, 50, 0, 0), new))
 
 
-@pytest.mark.parametrize("N", [1, 3, 90])
+@pytest.mark.parametrize("N", [1, 3, 7, 14, 20, 90])
 @pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16])
 def test_what_lies_behind_a_rows_last_key_does_not_touch_it(dt, N):
     cache = filled(24, 1, 16, 64, 3, spread=3)
@@ -167,15 +167,16 @@ def test_pages_that_hold_nothing_yet(N):
         assert torch.equal(fused_paged_attention(q, cache, bt, ints(100 - N)), want)
 
 
-def test_nan_in_a_value_reaches_its_dim_alone():
+@pytest.mark.parametrize("H", [1, 2, 4, 16])
+def test_nan_in_a_value_reaches_its_dim_alone(H):
     cache = filled(8, 1, 16, 64, 5)
     bt = tables(1, 8, 8, 5)
-    q = randn(6, 1, 4, 20, 64).bfloat16()
+    q = randn(6, 1, H, 20, 64).bfloat16()
     cache.v.view(torch.uint8)[bt[0, 1].long(), 0, 3, 7] = 0x7F     # key 19, seen by all rows
     cache.v.view(torch.uint8)[bt[0, 6].long(), 0, 4, 9] = 0xFF     # key 100, seen by tokens 10 on
     o = check_attend(q, cache, bt, ints(90))
     nan = torch.isnan(o[0])
-    assert nan[:, :, 7].all() and nan[:, 10:, 9].all() and int(nan.sum()) == 4 * 20 + 4 * 10
+    assert nan[:, :, 7].all() and nan[:, 10:, 9].all() and int(nan.sum()) == H * 20 + H * 10
 
 
 def test_pages_the_table_does_not_name():
@@ -193,7 +194,7 @@ def test_pages_the_table_does_not_name():
     assert torch.isnan(o[2]).all()
 
 
-@pytest.mark.parametrize("N", [1, 70])
+@pytest.mark.parametrize("N", [1, 12, 30, 50, 140])
 @pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16])
 def test_scales_far_apart_and_zero_pages(dt, N):
     """V pages at 2^-40 beside 2^10, pages of zeros (the least scale) among them, K scales apart too."""
