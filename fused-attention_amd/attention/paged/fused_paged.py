@@ -18,8 +18,8 @@ block_table: (B, pages) int32, the page that holds keys [i * page_size, (i + 1) 
 past_lens: (B,) int32, the tokens each sequence held before this step.
 new_lens: (B,) int32, how many of the N new tokens are real (None: all); the rest is padding.
 
-Pages that a call appends to must each belong to one sequence (copy a shared page first); full pages
-may be shared.  A page is begun anew when its first row is written.  Its scale is the least power of two that brings its
+Pages that a call appends to must each stand once in one sequence's row of the table (copy a shared page
+first); pages that are only read may be shared.  A page is begun anew when its first row is written.  Its scale is the least power of two that brings its
 largest value into e4m3's range, 2^-40 at least and 2^40 at most; when a later token needs a larger one,
 the rows already there are moved along, exactly but for values that become subnormal.  Infinities and NaN are stored
 as NaN.  A token whose page the table does not name (negative, too large, or past its last column) is

@@ -94,7 +94,9 @@ __device__ __forceinline__ Block block_of(const PagedArgs& a, int b, int rb, int
   x.rows = a.N * G;
   const int tok0 = x.r0 / G, tok1 = min(min((x.r0 + block_rows - 1) / G, a.N - 1), x.fresh - 1);
   x.lmin = x.past + tok0;                              // the last key that the first live row sees
-  x.keys = tok0 < x.fresh ? x.past + tok1 + 1 : 0;
+  // (a length past the table: its first key without a page makes the rows NaN, the rest need not be walked)
+  const long long named = (long long)a.cache.table_width * a.cache.page_size;
+  x.keys = tok0 < x.fresh ? (int)min((long long)(x.past + tok1 + 1), named + 1) : 0;
   return x;
 }
 

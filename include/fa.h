@@ -275,7 +275,7 @@ FA_API size_t fa_qk_norm_rotary_workspace_size(int B, int H, int H_kv, int N, in
  *   moved along (exactly, but for values that become subnormal).  A finite value past 448 2^40 becomes
  *   that, an infinity or NaN becomes NaN.  Rows behind the last new token keep their bytes.  A token whose page the table does not
  *   name (out of [0, num_pages), or past table_width) is not stored.  Pages that are written must
- *   belong to one sequence.
+ *   stand once in the table, in one sequence's row.
  * fa_paged_attention: query n of sequence b against keys 0 .. past_lens[b] + n of its pages, scale 1/sqrt(D)
  *   folded in scale_log2 as in fa_fwd; query head h reads K/V head h / (H / H_kv).  q, o: rows as above.
  *   Padding gets zeros (lse -inf).  lse: NULL or [B, H, N] fp32 in fa_fwd's units.  A key whose page the

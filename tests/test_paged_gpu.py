@@ -537,6 +537,36 @@ def test_captured_steps(N):
     assert not torch.isnan(graphs[1][1]).any()
 
 
+@pytest.mark.parametrize("N", [1, 5, 20, 60, 100])
+def test_c_entry_with_less_workspace(N):
+    """fa_paged_attention splits the keys less with a smaller workspace, and not at all without one."""
+    import ctypes
+    from attention import _lib
+    from test_serving_refusals import Cache, Rows
+    lib = _lib.load()
+    B, H, Hkv, D, ps, width = 2, 4, 2, 64, 16, 150
+    cache = filled(B * width, Hkv, ps, D, 60, spread=3)
+    bt = tables(B, width, B * width, 61)
+    past = ints(width * ps - N, 700)
+    q = randn(62, B, H, N, D).bfloat16()
+    want = check_attend(q, cache, bt, past, label=f"whole workspace N={N}")
+    need = lib.fa_paged_attention_workspace_size(B, H, Hkv, N, D, width * ps)
+    assert need > 0
+    c = Cache(*(t.data_ptr() for t in cache), bt.data_ptr(), width, width, B * width, ps, Hkv)
+    rows = lambda t: ctypes.byref(Rows(t.data_ptr(), *t.stride()[:3]))  # noqa: E731
+    ws = torch.empty(need, dtype=torch.uint8, device="cuda")
+    for size in (need, need // 2, need // 7, 0):
+        o = torch.full_like(q, 7.0)
+        code = lib.fa_paged_attention(rows(q), ctypes.byref(c), past.data_ptr(), None, rows(o), None, B, H, N, D, 1,
+                                      _lib.scale_log2(D), ws.data_ptr() if size else None, size,
+                                      torch.cuda.current_stream().cuda_stream)
+        assert code == _lib.FA_OK
+        if size == need:
+            assert torch.equal(o, want)
+        # two splits of the same sums: each within its bound of the exact value, twice 2^-9 of it and the output's rounding
+        assert bool(((o.float() - want.float()).abs() <= 2.0 ** -8 * 2 + 2.0 ** -7 * want.float().abs()).all())
+
+
 def test_two_streams_at_once():
     cache = filled(64, 2, 16, 64, 50, spread=3)
     bt = tables(2, 32, 64, 50)
