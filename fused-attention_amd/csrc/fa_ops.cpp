@@ -84,9 +84,10 @@ fa_rows rows(const Tensor& x) {
 
 // New rows of x's shape, laid out in memory as x is: by token (a packed projection's views) or by head.
 Tensor rows_like(const Tensor& x) {
-  if (x.size(1) > 1 && x.size(2) > 1 && x.stride(1) < x.stride(2))
-    return at::empty({x.size(0), x.size(2), x.size(1), x.size(3)}, x.options()).transpose(1, 2);
-  return at::empty(x.sizes(), x.options());
+  const int64_t B = x.size(0), H = x.size(1), N = x.size(2), D = x.size(3);
+  if (H > 1 && N > 1 && x.stride(1) < x.stride(2))
+    return at::empty_strided({B, H, N, D}, {N * H * D, D, H * D, 1}, x.options());
+  return at::empty({B, H, N, D}, x.options());
 }
 
 // The rotation of a call, and the tensors it points into.

@@ -140,6 +140,9 @@ __global__ __launch_bounds__(kRowThreads) void qk_dw_kernel(QkArgs a, int q_chun
 
 namespace {
 
+// Heads a workgroup takes: eight, fewer while the grid is under two workgroups to a CU (us at one / two / four: B=1
+// H=32 H_kv=8 N=1531 D=128 with three axes 9.3 / 8.6 / 9.1, N=700 5.7 / 5.8 / 7.1, B=2 H=H_kv=16 N=1000 D=64 5.7 / 6.1 /
+// 7.9: each workgroup reads its tokens' table rows again).
 struct Plan {
   int heads, q_chunks, chunks;
   long long token_blocks;
@@ -151,7 +154,7 @@ Plan plan_of(int B, int H, int Hkv, int N, int D) {
   p.token_blocks = ((long long)B * N + tokens - 1) / tokens;
   p.heads = 8;
   auto chunks = [&](int h) { return (h + p.heads - 1) / p.heads; };
-  while (p.heads > 1 && p.token_blocks * (chunks(H) + chunks(Hkv)) < 4LL * cu_count()) p.heads /= 2;
+  while (p.heads > 1 && p.token_blocks * (chunks(H) + chunks(Hkv)) < 2LL * cu_count()) p.heads /= 2;
   p.q_chunks = chunks(H);
   p.chunks = p.q_chunks + chunks(Hkv);
   return p;
