@@ -492,27 +492,31 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(PagedArgs a, int row
   __shared__ __attribute__((aligned(16))) float sums[PAR][D];
   const int Hkv = a.cache.H_kv, G = a.H / Hkv, rows = a.N * G;
   const int bh = blockIdx.x / rows, rr = blockIdx.x % rows, b = bh / Hkv, hk = bh % Hkv;
-  const Block x = block_of(a, b, rr / block_rows, G, block_rows);
-  const int per = split_keys(x.keys, a.nsplit, step);
-  if (per >= x.keys) return;
-  const int n = (x.keys + per - 1) / per;
   const long long block = (long long)bh * row_blocks + rr / block_rows;
   const int p = threadIdx.x / TR, d0 = threadIdx.x % TR * 4;
   const float* const src = part_row<D>(a, block, 0, rr % block_rows, block_rows);
   const int stride = block_rows * (D + 4);
-  // every wave takes the maximum and the sum of all (m', l), two splits to a lane; the first keeps the factors
+  // every wave takes the maximum and the sum of all (m', l), two splits to a lane; the first keeps the factors.
+  // (The loads reach all nsplit places, written or not, so that they do not wait for the lengths, which say how
+  // many count.)
   const int lane = threadIdx.x & 63;
   float m[2], l[2], M = -__FLT_MAX__, L = 0.f;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    const float* const ml = src + min(lane + 64 * i, n - 1) * stride + D;
-    m[i] = ml[0], l[i] = lane + 64 * i < n ? ml[1] : 0.f;
+    const float* const ml = src + min(lane + 64 * i, a.nsplit - 1) * stride + D;
+    m[i] = ml[0], l[i] = ml[1];
   }
-  // (the sums' loads do not wait for the factors)
   constexpr int AHEAD = kMaxSplit / PAR < 8 ? kMaxSplit / PAR : 8;
   f32x4 v[AHEAD];
 #pragma unroll
-  for (int i = 0; i < AHEAD; ++i) v[i] = gload_f32x4(src + min(p + i * PAR, n - 1) * stride + d0);
+  for (int i = 0; i < AHEAD; ++i) v[i] = gload_f32x4(src + min(p + i * PAR, a.nsplit - 1) * stride + d0);
+  const Block x = block_of(a, b, rr / block_rows, G, block_rows);
+  const int per = split_keys(x.keys, a.nsplit, step);
+  if (per >= x.keys) return;
+  const int n = (x.keys + per - 1) / per;
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    if (lane + 64 * i >= n) m[i] = -__FLT_MAX__, l[i] = 0.f;
   M = fmaxf(m[0], m[1]);
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) M = fmaxf(M, __shfl_xor(M, d));
@@ -566,20 +570,20 @@ __global__ __launch_bounds__(kJoinThreads) void join_few_kernel(PagedArgs a, int
   const long long i = (long long)blockIdx.x * (kJoinThreads / TR) + threadIdx.x / TR;   // (batch, K/V head), row
   if (i >= (long long)a.B * Hkv * rows) return;
   const int bh = i / rows, rr = i % rows, b = bh / Hkv, hk = bh % Hkv;
-  const Block x = block_of(a, b, rr / block_rows, G, block_rows);
-  const int per = split_keys(x.keys, a.nsplit, step);
-  if (per >= x.keys) return;
-  const int n = (x.keys + per - 1) / per;
   const float* const src = part_row<D>(a, (long long)bh * row_blocks + rr / block_rows, 0, rr % block_rows, block_rows);
   const int stride = block_rows * (D + 4), d0 = threadIdx.x % TR * 4;
   float m[kFewSplits], l[kFewSplits], M = -__FLT_MAX__, L = 0.f;
   f32x4 v[kFewSplits], o = f32x4{};
 #pragma unroll
   for (int s = 0; s < kFewSplits; ++s)
-    if (s < n) {
+    if (s < a.nsplit) {   // (written or not, as above)
       m[s] = src[s * stride + D], l[s] = src[s * stride + D + 1];
       v[s] = gload_f32x4(src + s * stride + d0);
     }
+  const Block x = block_of(a, b, rr / block_rows, G, block_rows);
+  const int per = split_keys(x.keys, a.nsplit, step);
+  if (per >= x.keys) return;
+  const int n = (x.keys + per - 1) / per;
 #pragma unroll
   for (int s = 0; s < kFewSplits; ++s)
     if (s < n) M = fmaxf(M, m[s]);
