@@ -36,7 +36,8 @@ def makefile_sched():
 def objects():
     """(family, etype, D, forward part, scheduler flags) of every object the Makefile builds:
     the D = 128 forward as its one-head part and its grouped part, the other forward slices
-    whole, the backward per slice, each under its group's scheduler options."""
+    whole, the backward per slice, each under its group's scheduler options, and the objects
+    that hold every slice of their kernels (etype "", D 0)."""
     sch = makefile_sched()
     out = []
     for e, d in SLICES:
@@ -45,7 +46,7 @@ def objects():
                     ("bwd", e, d, 0, sch["SCHED_BWD128"])]
         else:
             out += [("fwd", e, d, 0, sch["SCHED_FWD"]), ("bwd", e, d, 0, sch["SCHED_BWD"])]
-    return out
+    return out + [(f, "", 0, 0, []) for f in ("rotary", "paged", "paged_rows")]
 
 
 def sched_name(flags):
@@ -56,13 +57,17 @@ def sched_name(flags):
 
 def compile_slice(hipcc, family, etype, D, part, sched):
     et = "fa::BF16" if etype == "bf16" else "fa::F16"
-    if family == "fwd":
+    if not etype:
+        defs = []
+    elif family == "fwd":
         defs = [f"-DFA_FWD_PART={part}", f"-DFA_FWD_TABLE=fa_fwd_table_{etype}_{D}",
                 f"-DFA_FWD_TABLE_GROUPED=fa_fwd_table_{etype}_{D}_grouped"]
     else:
         defs = [f"-DFA_BWD_TABLE=fa_bwd_table_{etype}_{D}"]
     src = os.path.join(CSRC, f"fa_{family}.hip")
-    r = subprocess.run([hipcc, *FLAGS, *sched, f"-DFA_ETYPE={et}", f"-DFA_D={D}", *defs, src],
+    if etype:
+        defs += [f"-DFA_ETYPE={et}", f"-DFA_D={D}"]
+    r = subprocess.run([hipcc, *FLAGS, *sched, *defs, src],
                        capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"{src} ({etype}, D={D}, part {part}) failed:\n{r.stderr[-2000:]}")
@@ -107,7 +112,9 @@ HEADER = [
     "`fwd_kernel<E, D, rows per head, keys per tile, heads per workgroup, key groups, LSE>`,",
     "`dq_kernel<E, D, rows, keys>`, `dkdv_kernel<E, D, query rows per tile, keys per workgroup, per-row terms>`,",
     "`dkdv_pair_kernel<E, D, query rows per tile, keys per workgroup>` (D = 128 only),",
-    "`bwd_small_kernel<E, D>` (dQ and dK/dV of small grids).  Each forward and dQ instance names its waves per SIMD",
+    "`bwd_small_kernel<E, D>` (dQ and dK/dV of small grids),",
+    "`qk_fwd_kernel` / `qk_bwd_kernel<E, D, interleaved>`, `append_kernel<E, D, interleaved, passes, threads>`,",
+    "`attend_kernel<E, D, 16-row blocks>`, `rows_kernel<E, D, waves, parts of a tile>`.  Each forward and dQ instance names its waves per SIMD",
     "as minimum and maximum, so an occupancy of 2 may stand beside registers that allow 3.",
     "",
 ]
@@ -118,7 +125,7 @@ def main(argv=None):
     p.add_argument("--hipcc", default="/opt/rocm/bin/hipcc")
     p.add_argument("--out", default="")
     args = p.parse_args(argv)
-    jobs = sorted(objects(), key=lambda j: (j[0] != "fwd", j[1], -j[2], j[3]))
+    jobs = sorted(objects(), key=lambda j: (j[1] == "", j[0] != "fwd", j[1], -j[2], j[3]))
     with ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 4)) as ex:
         results = list(ex.map(lambda j: compile_slice(args.hipcc, *j), jobs))
     cols = FIELDS + ["Scheduler"]
