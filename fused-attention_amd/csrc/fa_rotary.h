@@ -48,6 +48,7 @@ template <int D, bool INTER>
 struct Turn {
   float c[8], s[8];  // own value's factor; partner's factor, with its sign
   int partner;       // lane that holds the partners (interleaved: none)
+  uint32_t turned;   // all ones; 0 where nothing turns, so a partner that is infinite or NaN has no say (0 times it is NaN)
 
   __device__ __forceinline__ static int partner_lane(const RotaryArgs& a, int lane, int d0) {
     if (INTER || d0 >= a.rotary_dim) return lane;
@@ -66,23 +67,17 @@ struct Turn {
     return (a.axes > 1 && pair >= a.section_end[0] ? 1 : 0) + (a.axes > 2 && pair >= a.section_end[1] ? 1 : 0);
   }
 
-  // Factors of token (b, n) for dims d0 .. d0 + 7.  A negative position leaves the row unturned
-  // (padding); one past the table gives NaN.
-  __device__ __forceinline__ void load(const RotaryArgs& a, int lane, int d0, int b, int n, long long base) {
-    partner = partner_lane(a, lane, d0);
-    const bool turned = a.table != nullptr && d0 < a.rotary_dim;
-    if (!turned) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) c[i] = 1.f, s[i] = 0.f;
-      return;
-    }
+  // Cosines and sines of the lane's pairs, from pair0 on, at token (b, n).  A negative position leaves the row
+  // unturned (padding); one past the table gives NaN.
+  template <int NP>
+  __device__ __forceinline__ void table_factors(const RotaryArgs& a, int pair0, int b, int n, long long base, float (&cc)[NP],
+                                                float (&ss)[NP]) {
     const int half = a.rotary_dim / 2;
-    constexpr int NP = INTER ? 4 : 8;   // pairs of this lane
-    const int pair0 = INTER ? d0 / 2 : (d0 < half ? d0 : d0 - half);
-    float cc[NP], ss[NP];
     const int axis = axis_of(a, pair0);
     const long long p = position(a, axis, b, n, base);
+    turned = ~0u;
     if (axis == axis_of(a, pair0 + NP - 1)) {
+      if (p < 0) turned = 0;
       const float* row = a.table + (p < 0 ? 0 : p >= a.table_len ? 0 : p) * a.rotary_dim + pair0;
 #pragma unroll
       for (int i = 0; i < NP; i += 4) {
@@ -119,6 +114,18 @@ struct Turn {
         ss[i] = at[i] < 0 ? 0.f : ss[i] + bad;
       }
     }
+  }
+
+  // Factors of token (b, n) for dims d0 .. d0 + 7.
+  __device__ __forceinline__ void load(const RotaryArgs& a, int lane, int d0, int b, int n, long long base) {
+    partner = partner_lane(a, lane, d0);
+    const int half = a.rotary_dim / 2;
+    constexpr int NP = INTER ? 4 : 8;   // pairs of this lane
+    float cc[NP], ss[NP];
+#pragma unroll
+    for (int i = 0; i < NP; ++i) cc[i] = 1.f, ss[i] = 0.f;
+    turned = 0;
+    if (a.table != nullptr && d0 < a.rotary_dim) table_factors(a, INTER ? d0 / 2 : (d0 < half ? d0 : d0 - half), b, n, base, cc, ss);
     if constexpr (INTER) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -133,12 +140,14 @@ struct Turn {
     }
   }
 
-  // The partner lane's packed row (its own when interleaved: the pairs are inside the lane).
+  // The partner lane's packed row (its own when interleaved: the pairs are inside the lane); zeros where nothing turns.
   __device__ __forceinline__ u32x4 fetch(const u32x4& w) const {
-    if constexpr (INTER) return w;
-    u32x4 r;
+    u32x4 r = w;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) r[i] = (uint32_t)__builtin_amdgcn_ds_bpermute(partner << 2, (int)w[i]);
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (!INTER) r[i] = (uint32_t)__builtin_amdgcn_ds_bpermute(partner << 2, (int)w[i]);
+      r[i] &= turned;
+    }
     return r;
   }
 };

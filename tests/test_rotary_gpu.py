@@ -291,3 +291,27 @@ def test_capture_is_refused_while_an_eager_graph_of_the_leaves_lives():
     torch.cuda.synchronize()
     del alive
     fused_qk_norm_rotary_autograd(*leaves, table)
+
+
+@pytest.mark.parametrize("it", [False, True])
+@pytest.mark.parametrize("bad", [float("inf"), float("nan")])
+def test_unturned_values_do_not_see_their_neighbours(it, bad):
+    """Dims past the rotated ones and rows at negative positions are handed on as they are, whatever
+    stands beside them, in the outputs and in the gradients."""
+    B, H, Hkv, N, D, R = 2, 3, 1, 5, 64, 32
+    q, k = (torch.randn(B, h, N, D, generator=gen(3), device="cuda").to(torch.bfloat16) for h in (H, Hkv))
+    dq, dk = (torch.randn(t.shape, generator=gen(4), device="cuda").to(t.dtype) for t in (q, k))
+    for t in (q, k, dq, dk):
+        t[..., 40] = bad                     # a neighbour in an unturned pair
+        t[:, :, 2, 1] = bad                  # and in the row that is not turned at all
+    table = rotary_table(16, R)
+    pos = torch.arange(N, device="cuda", dtype=torch.int32)
+    pos[2] = -1
+    leaves = [t.clone().requires_grad_(True) for t in (q, k)]
+    out = fused_qk_norm_rotary_autograd(*leaves, None, None, table, pos, None, EPS, it)
+    grads = torch.autograd.grad(out, leaves, (dq, dk))
+    for got, want in (*zip(out, (q, k)), *zip(grads, (dq, dk))):
+        for x, y in ((got[..., R:], want[..., R:]), (got[:, :, 2], want[:, :, 2])):
+            assert torch.equal(torch.nan_to_num(x.detach(), nan=12345.0), torch.nan_to_num(y, nan=12345.0))
+        live = [n for n in range(N) if n != 2]
+        assert bool(torch.isfinite(got[:, :, live, :R]).all())
