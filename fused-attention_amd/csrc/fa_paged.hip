@@ -45,7 +45,8 @@ __device__ __forceinline__ void decode8(const u32x2& w, float (&y)[8]) {
 // over the rows that the workgroup's NT threads hold at once; four at most, or the registers leave too few waves
 // (128-row pages at D = 128: eight passes of 256 threads 101 us, four of 512 95; 64-row pages: four of 256 90, two
 // of 512 91), and no more threads than a page has pieces (16-row pages at D = 64, B=3 N=1000: 256 threads 9.3 us,
-// 128 7.1).
+// 128 7.1).  Bytes bound the large call: B=2 H=32 H_kv=8 N=8192 D=128 in pages of 128 takes 93 us, 4.05 TB/s, some 12
+// of them K's norm and table rows; one token a sequence is the chain length, page, scale, row, code (B=64: 6.8 us).
 template <typename E, int D, bool INTER, int PASSES, int NT>
 __global__ __launch_bounds__(NT) void append_kernel(AppendArgs a, int items, int q_chunks, int touched) {
   using S = Slot<D, NT>;
@@ -178,6 +179,9 @@ __global__ __launch_bounds__(NT) void append_kernel(AppendArgs a, int items, int
 // 16-key tiles fill its 32 contraction slots; with slot (group g, j) = key 16 (j / 4) + 4 g + j % 4
 // no score moves between lanes, and V is read in that order, straight from the pages' rows: a lane
 // takes D / 16 dims of each of its 8 keys and pairs them up in registers.  Nothing is staged in LDS.
+// Bytes bound it: 32 sequences of 5461 to 16384 keys, H=32 H_kv=8 D=128, 136.6 us with the join, 5.3 TB/s; where
+// the bytes are few, the chain length, page, scale, keys and the join's launch do (8 sequences of up to 4005 keys:
+// 12.9 + 4.0 us for 47 MB).
 constexpr int kWaves = 4;
 constexpr int kRows = 16;
 constexpr int kStep = 32;   // keys per step of a wave

@@ -6,12 +6,14 @@
 // of one K/V head, so neighbouring rows share every key), walks the keys in tiles of 64, and keeps two
 // tiles of K (in the queries' type) and V (fp16) in LDS.  A tile's codes come to registers while the tile
 // before them is computed, are converted (2 codes an instruction) and written to LDS under the products of
-// the next step, and are read in the step after it: no wave waits for them between two products.  Products, layouts and order of a step are those of the causal
-// forward (fa_fwd.hip): S^T = K Q^T on 32x32x16 products with a lane owning one row, the scores fed
-// back as the B operand of O^T += V^T P^T, V^T read transposed from LDS, S(j + 1) under the softmax of
-// S(j).  What differs:
-//   * a 16-key part of a tile (the whole tile with pages of 64 keys or more) lies in one page: its K scale multiplies its scores, its V scale joins
-//     their exponent, and leaves the row sums again, part by part;
+// the next step, and are read in the step after it: no wave waits for them between two products.  8 waves and
+// 256 rows where there are as many: each converted tile serves twice the rows.  Products, layouts and order of a
+// step are those of the causal forward (fa_fwd.hip): S^T = K Q^T on 32x32x16 products with a lane owning one row,
+// the scores fed back as the B operand of O^T += V^T P^T, V^T read transposed from LDS, S(j + 1) under the softmax
+// of S(j).  B=2 H=32 H_kv=8, 2048 new tokens behind 6144, D=128: 424 us, 1135 TFLOP/s, the matrix pipes busy 56 % of
+// the time at 1.94 GHz.  What differs:
+//   * a 16-key part of a tile (the whole tile with pages of 64 keys or more) lies in one page: its K scale
+//     multiplies its scores, its V scale joins their exponent, and leaves the row sums again, part by part;
 //   * pages and scales of 16 tiles (64 with pages of 64 keys or more) at a time are kept one part to a lane
 //     and loaded a run ahead;
 //   * the diagonal starts at past_lens: tiles below it run without a mask; a value of V behind the last

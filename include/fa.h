@@ -7,8 +7,9 @@
  * keeps a pointer after it returns.  The library does hold one static device
  * array: the 64 MiB scratch behind fa_bwd_gqa_noalloc, which every device the
  * loaded library runs on carries (in its code object's memory) until the
- * process ends, whichever entry points a caller uses.  All tensors are dense,
- * row-major [B, heads, S, D] in device memory; LSE is dense [B, H, S] float32.
+ * process ends, whichever entry points a caller uses.  Tensors are dense,
+ * row-major [B, heads, S, D] in device memory (fa_rows: with strides of their
+ * own; fa_paged_cache: pages); LSE is dense [B, H, S] float32.
  *
  * Return value: FA_OK (0) or one of the negative FA_ERR_* codes below.
  * fa_strerror() turns a code into a static message.
@@ -273,16 +274,16 @@ FA_API size_t fa_qk_norm_rotary_workspace_size(int B, int H, int H_kv, int N, in
  *   Scale of a page and head: the least power of two 2^e, -40 <= e <= 40, with |x| <= 448 2^e for its finite
  *   values; a page whose first row is written starts anew, else e only grows, and the rows it holds are
  *   moved along (exactly, but for values that become subnormal).  A finite value past 448 2^40 becomes
- *   that, an infinity or NaN becomes NaN.  Rows behind the last new token keep their bytes.  A token whose page the table does not
- *   name (out of [0, num_pages), or past table_width) is not stored.  Pages that are written must
- *   stand once in the table, in one sequence's row.
+ *   that, an infinity or NaN becomes NaN.  Rows behind the last new token keep their bytes.  A token whose
+ *   page the table does not name (out of [0, num_pages), or past table_width) is not stored.  Pages that
+ *   are written must stand once in the table, in one sequence's row.
  * fa_paged_attention: query n of sequence b against keys 0 .. past_lens[b] + n of its pages, scale 1/sqrt(D)
  *   folded in scale_log2 as in fa_fwd; query head h reads K/V head h / (H / H_kv).  q, o: rows as above.
  *   Padding gets zeros (lse -inf).  lse: NULL or [B, H, N] fp32 in fa_fwd's units.  A key whose page the
  *   table does not name makes the rows that see it NaN.  What lies behind a row's last key does not
  *   touch it, NaN included.
- *   workspace: fa_paged_attention_workspace_size() bytes, 16-byte aligned, for the partial rows of keys
- *   split over workgroups; with less (NULL) they are split less or not at all.
+ *   workspace: fa_paged_attention_workspace_size() bytes (keys: table_width * page_size), 16-byte aligned, for the
+ *   partial rows of keys split over workgroups; with less (NULL) they are split less or not at all.
  */
 typedef struct fa_paged_cache {
   void* k;

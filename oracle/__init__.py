@@ -10,6 +10,8 @@ Modules
                     online-softmax algorithm, and a pure-Python loop version
   cases             the reference's seeded correctness-case generators
   cpu_reference     the reference's PyTorch fp32 path (chunked), timed as the CPU baseline
+  paged_oracle      norm + rotation and its gradients, the 8-bit paged cache's append and the
+                    attention over it, in torch float64
 
 Parity pinning (every function is checked by tests/test_oracle.py against
 something other than a retyped formula):
@@ -34,5 +36,11 @@ cpu_reference (tests/test_cpu_reference.py) is pinned against the float64 oracle
                     K/V head index, chunks straddling a group, the last K/V head rounded
                     down, a shifted output slice) are caught
   fp32 autograd     dQ, dK, dV for MHA and GQA (group sums), the single 1/sqrt(D) factor
+paged_oracle (tests/test_paged_oracle.py):
+  rotation          complex multiplication; scores depend on the distance of positions alone
+  gradients         central differences and torch autograd in float64
+  e4m3, scales      torch's cast at every representable midpoint; the least exponent that fits
+  attention         torch SDPA in float64 over the decoded pages; planted mistakes show
+  append            decoding returns each value rounded
 No function is left "parity unpinned".
 """
