@@ -245,7 +245,8 @@ void rows_kernel(PagedArgs a, int row_blocks) {
   // taken out.  Both in fp32 from p as it is: where scales lie far apart a key that counts may have a p' that
   // fp16 rounds to nothing.  (On the matrix pipe, from P as rounded, the sums would also hang on the other rows
   // of their column: its zeros hand on a NaN.)
-  auto exp_tile = [&](const f32x16 (&s)[NB], int t, u32x4 (&pk)[2 * NB], float& l) __attribute__((always_inline)) {
+  // (Masked: a key that the row does not see counts for nothing, also where it has no page and its scale is NaN.)
+  auto exp_tile = [&](const f32x16 (&s)[NB], int t, u32x4 (&pk)[2 * NB], float& l, auto full) __attribute__((always_inline)) {
     float sum = 0.f;
     l = 0.f;
 #pragma unroll
@@ -257,7 +258,11 @@ void rows_kernel(PagedArgs a, int row_blocks) {
       for (int i = 2 * NB / PPT * k; i < 2 * NB / PPT * (k + 1); ++i) {
         float p[8];
 #pragma unroll
-        for (int g = 0; g < 8; ++g) p[g] = fast_exp2(__builtin_fmaf(s[i / 2][8 * (i & 1) + g], ks, off));
+        for (int g = 0; g < 8; ++g) {
+          const float x = s[i / 2][8 * (i & 1) + g];
+          p[g] = fast_exp2(__builtin_fmaf(x, ks, off));
+          if (!decltype(full)::value && x == NEG_INF) p[g] = 0.f;
+        }
 #pragma unroll
         for (int q = 0; q < 4; ++q) pk[i][q] = pack2<F16>(p[2 * q], p[2 * q + 1]);
         y += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
@@ -267,12 +272,12 @@ void rows_kernel(PagedArgs a, int row_blocks) {
     }
     return sum;
   };
-  auto softmax = [&](const f32x16 (&s)[NB], int t, u32x4 (&pk)[2 * NB]) __attribute__((always_inline)) {
+  auto softmax = [&](const f32x16 (&s)[NB], int t, u32x4 (&pk)[2 * NB], auto full) __attribute__((always_inline)) {
     float l;
-    const float sum = exp_tile(s, t, pk, l);
+    const float sum = exp_tile(s, t, pk, l, full);
     if (__builtin_amdgcn_ballot_w64(!(sum <= kRowSumLimit))) {
       rescale_to(tile_max(s, t));
-      exp_tile(s, t, pk, l);
+      exp_tile(s, t, pk, l, full);
     }
     lsum += l;
   };
@@ -335,7 +340,7 @@ void rows_kernel(PagedArgs a, int row_blocks) {
       s_tile(kcur, sn);
       if constexpr (!FULL) mask_tile(sn, first + (j + 1) * BN);
       pv_pre(vcur);
-      softmax(sc, j, pk);
+      softmax(sc, j, pk, full);
       pv_full(vcur, pk);
     };
     auto iteration = [&](int j, f32x16 (&sc)[NB], f32x16 (&sn)[NB], auto full) __attribute__((always_inline)) {
@@ -366,7 +371,7 @@ void rows_kernel(PagedArgs a, int row_blocks) {
     __syncthreads();
     u32x4 pk[2 * NB];
     pv_pre(Vbuf(j));
-    softmax(sa, j, pk);
+    softmax(sa, j, pk, Flag<false>{});
     pv_full(Vbuf(j), pk);
 
     if (__builtin_amdgcn_readfirstlane(nan_met) != 0) {

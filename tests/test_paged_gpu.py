@@ -601,3 +601,17 @@ def test_random_calls():
         q, k, v = (t.transpose(1, 2) for t in x.split((G * Hkv, Hkv, Hkv), 2))
         q = append_paged_kv(cache, k, v, bt, ints(*lens), ints(*new), q, None, None, rotary_table(600, D))
         check_attend(q, cache, bt, ints(*lens), ints(*new), label=f"random {i}")
+
+
+@pytest.mark.parametrize("N,D,ps", [(70, 64, 16), (150, 128, 32), (140, 32, 64), (300, 128, 128)])
+def test_prompt_over_a_page_without_a_name(N, D, ps):
+    """Rows before its first key do not see it, though their tile holds it."""
+    width = (N + 20 + ps - 1) // ps
+    cache = filled(width, 1, ps, D, 70)
+    bt = tables(1, width, width, 71)
+    bt[0, (20 + N // 2) // ps] = -1
+    q = randn(72, 1, 2, N, D).bfloat16()
+    o = check_attend(q, cache, bt, ints(20))
+    first = max((20 + N // 2) // ps * ps - 20, 0)   # the first row that sees a key of that page
+    nan = torch.isnan(o)
+    assert not nan[0, :, :first].any() and nan[0, :, first:].all()
