@@ -49,6 +49,7 @@ SIGNATURES = {
     "fa_qk_norm_rotary_workspace_size": (ctypes.c_size_t, [_I, _I, _I, _I, _I]),
     "fa_paged_append": (_I, [_VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _I, _I, _I, _I, _I, _VP]),
     "fa_paged_attention": (_I, [_VP, _VP, _VP, _VP, _VP, _VP, _I, _I, _I, _I, _I, _F, _VP, ctypes.c_size_t, _VP]),
+    "fa_paged_attention_exact": (_I, [_VP, _VP, _VP, _VP, _VP, _VP, _I, _I, _I, _I, _I, _F, _I, _I, _VP, ctypes.c_size_t, _VP]),
     "fa_paged_attention_workspace_size": (ctypes.c_size_t, [_I, _I, _I, _I, _I, ctypes.c_longlong]),
     "fa_noalloc_scratch_bytes": (ctypes.c_size_t, []),
     "fa_fwd_exact": (_I, [_VP, _VP, _VP, _VP, _VP, _I, _I, _I, _I, _I, _I, _F, _I, _I, _I, _VP]),

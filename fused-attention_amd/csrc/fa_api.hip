@@ -111,6 +111,23 @@ int check_cache(const fa_paged_cache& c) {
   return aligned16(c.k) && aligned16(c.v) ? FA_OK : FA_ERR_PAGES;
 }
 
+// Checks a call's arguments and fills `a`.
+int paged_args(fa::PagedArgs& a, const fa_rows* q, const fa_paged_cache* cache, const int* past_lens, const int* new_lens,
+               const fa_rows* o, float* lse, int B, int H, int N, int D, int dtype, float scale_log2, void* workspace,
+               void* hip_stream) {
+  if (!q || !o || !cache || !past_lens) return FA_ERR_NULL;
+  int st = check_cache(*cache);
+  if (st == FA_OK) st = check_rows_call(B, H, cache->H_kv, N, D, dtype);
+  if (st != FA_OK) return st;
+  if (H % cache->H_kv != 0) return FA_ERR_DIMS;
+  if ((st = check_rows(*q)) != FA_OK || (st = check_rows(*o)) != FA_OK) return st;
+  if (!aligned16(workspace)) return FA_ERR_WORKSPACE;
+  a.q = *q, a.o = *o, a.cache = *cache, a.past = past_lens, a.fresh = new_lens, a.lse = lse;
+  a.part = static_cast<float*>(workspace);
+  a.B = B, a.H = H, a.N = N, a.D = D, a.scale_log2 = scale_log2, a.stream = hip_stream;
+  return FA_OK;
+}
+
 using fa::cu_count;
 using fa::kMaxDevices;
 
@@ -602,18 +619,18 @@ int fa_paged_append(const fa_rows* q, const fa_rows* k, const fa_rows* v, const 
 int fa_paged_attention(const fa_rows* q, const fa_paged_cache* cache, const int* past_lens,
                        const int* new_lens, const fa_rows* o, float* lse, int B, int H, int N, int D,
                        int dtype, float scale_log2, void* workspace, size_t workspace_bytes, void* hip_stream) {
-  if (!q || !o || !cache || !past_lens) return FA_ERR_NULL;
-  int st = check_cache(*cache);
-  if (st == FA_OK) st = check_rows_call(B, H, cache->H_kv, N, D, dtype);
-  if (st != FA_OK) return st;
-  if (H % cache->H_kv != 0) return FA_ERR_DIMS;
-  if ((st = check_rows(*q)) != FA_OK || (st = check_rows(*o)) != FA_OK) return st;
-  if (reinterpret_cast<uintptr_t>(workspace) & 15) return FA_ERR_WORKSPACE;
   fa::PagedArgs a{};
-  a.q = *q, a.o = *o, a.cache = *cache, a.past = past_lens, a.fresh = new_lens, a.lse = lse;
-  a.part = static_cast<float*>(workspace);
-  a.B = B, a.H = H, a.N = N, a.D = D, a.scale_log2 = scale_log2, a.stream = hip_stream;
-  return fa::paged_attention(dtype, a, workspace ? workspace_bytes : 0);
+  const int st = paged_args(a, q, cache, past_lens, new_lens, o, lse, B, H, N, D, dtype, scale_log2, workspace, hip_stream);
+  return st != FA_OK ? st : fa::paged_attention(dtype, a, workspace ? workspace_bytes : 0);
+}
+
+int fa_paged_attention_exact(const fa_rows* q, const fa_paged_cache* cache, const int* past_lens,
+                             const int* new_lens, const fa_rows* o, float* lse, int B, int H, int N, int D,
+                             int dtype, float scale_log2, int block_rows, int parts, void* workspace,
+                             size_t workspace_bytes, void* hip_stream) {
+  fa::PagedArgs a{};
+  const int st = paged_args(a, q, cache, past_lens, new_lens, o, lse, B, H, N, D, dtype, scale_log2, workspace, hip_stream);
+  return st != FA_OK ? st : fa::paged_attention_exact(dtype, a, block_rows, parts, workspace ? workspace_bytes : 0);
 }
 
 size_t fa_paged_attention_workspace_size(int B, int H, int H_kv, int N, int D, long long keys) {

@@ -105,6 +105,7 @@ int qk_norm_rotary_bwd(int dtype, int D, const QkArgs& a);
 size_t qk_norm_rotary_workspace(int B, int H, int Hkv, int N, int D);
 int paged_append(int dtype, const AppendArgs& a);
 int paged_attention(int dtype, PagedArgs a, size_t workspace_bytes);
+int paged_attention_exact(int dtype, PagedArgs a, int block_rows, int parts, size_t workspace_bytes);
 size_t paged_attention_workspace(int B, int H, int Hkv, int N, int D, long long keys);
 
 // Raise the dynamic LDS limit of a kernel once (needed above 64 KB).  The

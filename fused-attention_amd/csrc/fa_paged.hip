@@ -4,6 +4,7 @@
 #include "fa_rotary.h"
 
 #include <algorithm>
+#include <iterator>
 
 namespace fa {
 
@@ -173,8 +174,8 @@ __global__ __launch_bounds__(NT) void append_kernel(AppendArgs a, int items, int
 // ---------------------------------------------------------------------------
 // Attention of few rows (the mathematics: fa_paged.h).
 //
-// Rows: the N x G queries of a K/V head (G = H / H_kv), row r = token r / G, head r % G: 16, 32 or 64
-// to a workgroup, so each key's bytes serve all of them.  S^T = K Q^T as 16x16x32 products (16 keys x 16
+// Rows: the N x G queries of a K/V head (G = H / H_kv), row r = token r / G, head r % G: 16 or 32 to
+// a workgroup, so each key's bytes serve all of them.  S^T = K Q^T as 16x16x32 products (16 keys x 16
 // rows): a lane owns one row, and the scores are fed back as the B operand of O^T += V^T P^T.  Two
 // 16-key tiles fill its 32 contraction slots; with slot (group g, j) = key 16 (j / 4) + 4 g + j % 4
 // no score moves between lanes, and V is read in that order, straight from the pages' rows: a lane
@@ -239,9 +240,15 @@ struct Tile {
   }
 };
 
+// Workgroups reach the XCDs in turn (wg % 8).  Where the parts of all units' keys fill the XCDs evenly, the row blocks of
+// one part go to one XCD, whose L2 then reads those keys once (8 sequences of 4000 keys, 8 K/V heads, D = 128, four
+// blocks of 16 rows 47.4 -> 26.8 us; two parts alone, 250 blocks: 25.9 -> 57 on two XCDs).  The parts take turns: a
+// run of them to each XCD leaves those with the shorter sequences idle (32 sequences of 5461 to 16384 keys 137 -> 154).
+__host__ __device__ __forceinline__ bool by_xcd(long long parts) { return parts % 8 == 0 || parts >= 64; }
+
 // RT: 16-row blocks that a wave holds; each converted K and V operand serves all of them.
 template <typename E, int D, int RT>
-__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(RT <= 2 ? 2 : 1))) void attend_kernel(PagedArgs a, int row_blocks) {
+__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2))) void attend_kernel(PagedArgs a, int row_blocks) {
   typedef Tile<D> T;
   constexpr int VB = T::VB;
   constexpr int KT = D / 32;         // contraction steps over D
@@ -254,9 +261,14 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(RT 
   const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int Hkv = a.cache.H_kv, ps = a.cache.page_size, G = a.H / Hkv;
-  const int split = blockIdx.x % a.nsplit;
-  const long long block = blockIdx.x / a.nsplit;
-  const int rb = block % row_blocks, bh = block / row_blocks;
+  const int parts = a.B * Hkv * a.nsplit;   // of all units' keys
+  int part = blockIdx.x / row_blocks, rb = row_blocks - 1 - blockIdx.x % row_blocks;   // (the most keys first)
+  if (by_xcd(parts)) {   // (the grid is whole rounds of 8 parts)
+    part = blockIdx.x / (8 * row_blocks) * 8 + blockIdx.x % 8, rb = row_blocks - 1 - blockIdx.x / 8 % row_blocks;
+    if (part >= parts) return;
+  }
+  const int split = part % a.nsplit, bh = part / a.nsplit;
+  const long long block = (long long)bh * row_blocks + rb;
   const int b = bh / Hkv, hk = bh % Hkv;
   const Block x = block_of(a, b, rb, G, BR);
   const int per = split_keys(x.keys, a.nsplit, kSplitStep);
@@ -647,49 +659,63 @@ int launch_append(const AppendArgs& a) {
   return FA_ERR_UNSUPPORTED;
 }
 
-// How a call's rows and keys are cut: blocks of `rows` rows, each block's keys in up to nsplit parts of
-// whole `step`s.  Only the lengths' bound (the table's width) is known here; a shorter sequence takes
-// fewer parts (split_keys).
+// How a call's rows and keys are cut: blocks of `rows` rows (16 and 32 to the kernel of few rows), each block's
+// keys in up to nsplit parts of whole `step`s.  Only the lengths' bound (the table's width) is known here; a shorter
+// sequence takes fewer parts (split_keys).
 struct Cut {
   int rows, step, row_blocks, nsplit;
 };
 
-// Few rows: as many parts as give each CU a workgroup (more only divide the same bytes into shorter runs
-// and more partial rows: us at 1 / 2 / 4 workgroups to a CU, 8 sequences of 1335 to 4005 keys, 8 K/V heads, D = 128:
-// 17.4 / 20.7 / 26.4; 64 of 667 to 2000 keys 36.1 / 36.2 / 40.8; one of 16000 keys 13.8 / 15.5 / 24.9), up to
+// Up to 16 rows, a token or a few: as many parts as give each CU a workgroup (more only divide the same bytes into
+// shorter runs and more partial rows: us at 1 / 2 / 4 workgroups to a CU, 8 sequences of 1335 to 4005 keys, 8 K/V heads,
+// D = 128: 17.4 / 20.7 / 26.4; 64 of 667 to 2000 keys 36.1 / 36.2 / 40.8; one of 16000 keys 13.8 / 15.5 / 24.9), up to
 // four where a part keeps 4096 keys, for lengths that differ (32 sequences of 5461 to 16384 keys 140.9 / 141.9 / 135.3).
-// Up to 64 rows go to the kernel of few rows, in one block of 16, 32 or 64 (us of blocks of 16 / 32 / 64 / 128-row
-// workgroups; 8 sequences of 4000 keys, 8 K/V heads, D = 128: 32 rows 28 / 21 / - / 32, 64 rows 38 / - / 28 / 34), but
-// in two of 16 where the parts of one would not reach all CUs (one K/V head, 16384 keys, D = 64, 32 rows: 8.7 against
-// 9.6 in one block); 128 rows to 128-row workgroups, more to 256-row ones (us of 128 / 256 rows: 128 rows 40 / 46, 256
-// rows 60 / 58, 512 rows 93 / 91).  Their parts are those of the least cost by the times that a tile of one
-// workgroup to a CU, a workgroup's start and the join of its partial rows take.
+//
+// More rows: the shape and the parts of the least cost by the times below: a workgroup's start, a step of its keys where
+// each CU holds one workgroup, and on a full CU what each workgroup adds, a step and by itself; the read of the keys;
+// the join with its partial rows.  They come within 15 % (rms) of the good ones among 1500 cuts of 150 calls (2 to 3000
+// new tokens, D = 32, 64 and 128), and the cut taken is 2 % slower than the best of its call on average, 22 % at most.
+// Small blocks spread a short prompt over the CUs, large ones convert each key for more rows (us of blocks of 16 / 32 / 128 / 256
+// rows, D = 128, one sequence, H=32 H_kv=8, no keys before: 64 new tokens 6.4 / 7.7 / 7.4 / 9.4, 512 18.2 / 14.0 / 16.7 /
+// 20.5, 2048 119 / 75 / 53 / 57; two of 2048 235 / 151 / 87 / 77; blocks of 64 rows on four waves lay behind one of the
+// others everywhere).
+struct Shape {
+  int rows, step;
+  float start, one, full, each;   // us; steps at D = 128
+};
+constexpr Shape kShapes[] = {{16, kSplitStep, 6.f, 0.8f, 0.8f, 0.7f},
+                             {32, kSplitStep, 7.f, 0.9f, 1.0f, 0.7f},
+                             {128, kBlockKeys, 6.5f, 1.2f, 1.05f, 0.7f},
+                             {256, kBlockKeys, 7.f, 1.8f, 1.9f, 3.0f}};
+constexpr int kParts[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64, 96, kMaxSplit};
+
 Cut cut_of(int B, int H, int Hkv, int N, int D, long long keys) {
-  Cut c;
   const long long rows = (long long)N * (H / Hkv), units = (long long)B * Hkv;
   const long long cus = cu_count();
-  c.rows = 16;
-  while (c.rows < rows && c.rows < 256) c.rows *= 2;
-  if (c.rows == 32 && units * (keys / kSplitStep) < cus) c.rows = 16;
-  c.row_blocks = (int)((rows + c.rows - 1) / c.rows);
-  const long long blocks = units * c.row_blocks;
-  if (c.rows <= 64) {
-    c.step = kSplitStep;
-    const long long fill = (cus + blocks - 1) / blocks, four = (4 * cus + blocks - 1) / blocks;
+  Cut c{16, kSplitStep, 1, 1};
+  if (rows <= 16) {
+    const long long fill = (cus + units - 1) / units, four = (4 * cus + units - 1) / units;
     c.nsplit = (int)std::max<long long>(1, std::min<long long>({std::max(fill, std::min(four, keys / 4096)),
                                                                 (keys + c.step - 1) / c.step, kMaxSplit}));
     return c;
   }
-  c.step = kBlockKeys;
-  const long long tiles = (keys + kBlockKeys - 1) / kBlockKeys;
-  const float tile_us = (c.rows == 128 ? 1.7f : 2.2f) * (D + 32) / 160.f;
+  const float seen = 1.f - 0.5f * (float)std::min<long long>(N, keys) / (float)keys;   // of the keys, by a row on average
+  const float read = (float)(units * keys) * (float)D * (2.f / 7.0e6f);                // us at 7 TB/s, part of it from caches
+  const float wide = (float)(D + 32) / 160.f, row_values = 2.5e-6f * (float)(units * rows) * (float)D;
   float best = 0.f;
-  c.nsplit = 1;
-  for (int n = 1; n <= kMaxSplit && n <= tiles; n += n < 16 ? 1 : 8) {
-    const long long rounds = (blocks * n + cus - 1) / cus;
-    const float join = n == 1 ? 0.f : 3.f + 8e-6f / 3.f * (float)(units * rows) * (float)D * (float)n;
-    const float us = (float)rounds * (2.f + tile_us * (float)((tiles + n - 1) / n)) + join;
-    if (n == 1 || us < best) best = us, c.nsplit = n;
+  for (const Shape& s : kShapes) {
+    if (s.rows >= 2 * rows) break;
+    const long long blocks = (rows + s.rows - 1) / s.rows;
+    const unsigned most = (unsigned)std::min<long long>((keys + s.step - 1) / s.step, 1u << 30);
+    for (const int n : kParts) {
+      const long long wgs = units * blocks * n;
+      if (n > 1 && ((unsigned)n > most || wgs > 4 * cus)) break;
+      const float load = (float)wgs / (float)cus, steps = (float)((most + n - 1) / n) * wide;
+      const float on_cu = s.rows <= 32 ? load : (float)(long long)(load + 0.999f);   // (one of the large at a time)
+      const float work = std::max({steps * s.one, (steps * seen * s.full + s.each) * on_cu, read});
+      const float us = s.start + work + (n == 1 ? 0.f : 2.5f + row_values * (float)n);
+      if (best == 0.f || us < best) best = us, c = Cut{s.rows, s.step, (int)blocks, n};
+    }
   }
   return c;
 }
@@ -700,17 +726,16 @@ size_t part_bytes(int B, int Hkv, const Cut& c, int D) {
 
 template <typename E, int D>
 int launch_attend(const PagedArgs& a, const Cut& c, int dtype) {
-  const long long grid = (long long)a.B * a.cache.H_kv * c.row_blocks * a.nsplit;
+  const long long parts = (long long)a.B * a.cache.H_kv * a.nsplit;
+  const long long grid = (c.rows <= 32 && by_xcd(parts) ? (parts + 7) / 8 * 8 : parts) * c.row_blocks;
   const long long joins = (long long)a.B * a.H * a.N;
-  if (!grid_fits(grid, c.rows <= 64 ? 64 * kWaves : 2 * c.rows)) return FA_ERR_DIMS;
+  if (!grid_fits(grid, c.rows <= 32 ? 64 * kWaves : 2 * c.rows)) return FA_ERR_DIMS;
   if (a.nsplit > kFewSplits && !grid_fits(joins, kJoinThreads)) return FA_ERR_DIMS;
   hipStream_t st = (hipStream_t)a.stream;
   if (c.rows == 16) {
     hipLaunchKernelGGL((attend_kernel<E, D, 1>), dim3((unsigned)grid), dim3(64 * kWaves), 0, st, a, c.row_blocks);
   } else if (c.rows == 32) {
     hipLaunchKernelGGL((attend_kernel<E, D, 2>), dim3((unsigned)grid), dim3(64 * kWaves), 0, st, a, c.row_blocks);
-  } else if (c.rows == 64) {
-    hipLaunchKernelGGL((attend_kernel<E, D, 4>), dim3((unsigned)grid), dim3(64 * kWaves), 0, st, a, c.row_blocks);
   } else {
     const int status = paged_rows(dtype, a, c.row_blocks, c.rows);
     if (status != FA_OK) return status;
@@ -721,6 +746,18 @@ int launch_attend(const PagedArgs& a, const Cut& c, int dtype) {
     hipLaunchKernelGGL((join_few_kernel<E, D>), dim3((unsigned)((joins + 1024 / D - 1) / (1024 / D))), dim3(kJoinThreads), 0,
                        st, a, c.row_blocks, c.rows, c.step);
   return hipGetLastError() == hipSuccess ? FA_OK : FA_ERR_LAUNCH;
+}
+
+int attend(int dtype, PagedArgs a, const Cut& c) {
+  a.nsplit = c.nsplit;
+  if (dtype == FA_BF16) {
+    if (a.D == 32) return launch_attend<BF16, 32>(a, c, dtype);
+    if (a.D == 64) return launch_attend<BF16, 64>(a, c, dtype);
+    return launch_attend<BF16, 128>(a, c, dtype);
+  }
+  if (a.D == 32) return launch_attend<F16, 32>(a, c, dtype);
+  if (a.D == 64) return launch_attend<F16, 64>(a, c, dtype);
+  return launch_attend<F16, 128>(a, c, dtype);
 }
 
 }  // namespace
@@ -740,15 +777,16 @@ int paged_attention(int dtype, PagedArgs a, size_t workspace_bytes) {
   const int Hkv = a.cache.H_kv;
   Cut c = cut_of(a.B, a.H, Hkv, a.N, a.D, (long long)a.cache.table_width * a.cache.page_size);
   while (c.nsplit > 1 && part_bytes(a.B, Hkv, c, a.D) > workspace_bytes) --c.nsplit;
-  a.nsplit = c.nsplit;
-  if (dtype == FA_BF16) {
-    if (a.D == 32) return launch_attend<BF16, 32>(a, c, dtype);
-    if (a.D == 64) return launch_attend<BF16, 64>(a, c, dtype);
-    return launch_attend<BF16, 128>(a, c, dtype);
-  }
-  if (a.D == 32) return launch_attend<F16, 32>(a, c, dtype);
-  if (a.D == 64) return launch_attend<F16, 64>(a, c, dtype);
-  return launch_attend<F16, 128>(a, c, dtype);
+  return attend(dtype, a, c);
+}
+
+int paged_attention_exact(int dtype, PagedArgs a, int block_rows, int parts, size_t workspace_bytes) {
+  const Shape* const s = std::find_if(std::begin(kShapes), std::end(kShapes), [&](const Shape& x) { return x.rows == block_rows; });
+  if (s == std::end(kShapes)) return FA_ERR_TILE;
+  if (parts < 1 || parts > kMaxSplit) return FA_ERR_UNSUPPORTED;
+  const long long rows = (long long)a.N * (a.H / a.cache.H_kv);
+  const Cut c{block_rows, s->step, (int)((rows + block_rows - 1) / block_rows), parts};
+  return part_bytes(a.B, a.cache.H_kv, c, a.D) > workspace_bytes ? FA_ERR_WORKSPACE : attend(dtype, a, c);
 }
 
 size_t paged_attention_workspace(int B, int H, int Hkv, int N, int D, long long keys) {

@@ -303,6 +303,17 @@ FA_API int fa_paged_attention(const fa_rows* q, const fa_paged_cache* cache, con
                        int dtype, float scale_log2, void* workspace, size_t workspace_bytes, void* hip_stream);
 FA_API size_t fa_paged_attention_workspace_size(int B, int H, int H_kv, int N, int D, long long keys);
 
+/*
+ * fa_paged_attention with exactly the requested cut, for studies of the rule and tests of every kernel at every
+ * size: blocks of block_rows rows (16, 32, 128 or 256; else FA_ERR_TILE), each block's keys in up to `parts` parts
+ * (1 to 128).  workspace: FA_ERR_WORKSPACE below B * H_kv * ceil(N (H / H_kv) / block_rows) * parts * block_rows
+ * * (D + 4) * 4 bytes (one part: none).  fa_paged_attention picks both.
+ */
+FA_API int fa_paged_attention_exact(const fa_rows* q, const fa_paged_cache* cache, const int* past_lens,
+                             const int* new_lens, const fa_rows* o, float* lse, int B, int H, int N, int D,
+                             int dtype, float scale_log2, int block_rows, int parts, void* workspace,
+                             size_t workspace_bytes, void* hip_stream);
+
 /* 1 if a forward (with_lse 0/1) or backward (is_bwd 1) kernel exists for the
  * combination, else 0.  No reference counterpart: it lets a caller probe the
  * supported (dtype, D, tile) set before validating inputs. */

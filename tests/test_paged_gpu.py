@@ -615,3 +615,57 @@ def test_prompt_over_a_page_without_a_name(N, D, ps):
     first = max((20 + N // 2) // ps * ps - 20, 0)   # the first row that sees a key of that page
     nan = torch.isnan(o)
     assert not nan[0, :, :first].any() and nan[0, :, first:].all()
+
+
+def exact_cut(rows, parts):
+    """fused_paged_attention through the entry that takes one cut at every size."""
+    import ctypes
+    from attention import _lib
+    from test_serving_refusals import Cache, Rows
+    lib = _lib.load()
+
+    def call(q, cache, bt, past, new=None, return_lse=False):
+        B, H, N, D = q.shape
+        Hkv, ps = cache.k.shape[1:3]
+        bt, o = bt.contiguous(), torch.full_like(q, 7.0)
+        lse = torch.full((B, H, N), 7.0, device="cuda")
+        c = Cache(*(t.data_ptr() for t in cache), bt.data_ptr(), bt.shape[1], bt.shape[1], cache.k.shape[0], ps, Hkv)
+        size = 0 if parts == 1 else B * Hkv * -(-N * (H // Hkv) // rows) * parts * rows * (D + 4) * 4
+        ws = torch.full((size,), 255, dtype=torch.uint8, device="cuda")
+        at = lambda t: ctypes.byref(Rows(t.data_ptr(), *t.stride()[:3]))  # noqa: E731
+        assert lib.fa_paged_attention_exact(
+            at(q), ctypes.byref(c), past.data_ptr(), new.data_ptr() if new is not None else None, at(o), lse.data_ptr(),
+            B, H, N, D, int(q.dtype == torch.bfloat16), _lib.scale_log2(D), rows, parts, ws.data_ptr() if size else None,
+            size, torch.cuda.current_stream().cuda_stream) == _lib.FA_OK
+        return (o, lse) if return_lse else o
+    return call
+
+
+@pytest.mark.parametrize("parts", [1, 2, 5, 20])
+@pytest.mark.parametrize("rows", [16, 32, 128, 256])
+def test_every_cut_at_every_size(rows, parts, monkeypatch):
+    """What the tests above hold the chosen cut to, of each block size and number of parts."""
+    monkeypatch.setitem(globals(), "fused_paged_attention", exact_cut(rows, parts))
+    for D in (32, 64, 128):
+        for dt in (torch.float16, torch.bfloat16):
+            for ps in (16, 32, 64, 128):
+                test_attention_types_and_pages(D, dt, ps)
+    for H, Hkv, N in ((5, 5, 33), (8, 1, 7), (24, 8, 150), (32, 1, 20)):
+        test_attention_heads_and_rows(H, Hkv, N)
+    for total in (1, 31, 64, 129, 257, 700, 1500):
+        test_attention_lengths(total)
+    for N in (4, 18, 100):
+        test_padded_batch_and_empty_sequences(N)
+    for N in (1, 14, 90):
+        test_what_lies_behind_a_rows_last_key_does_not_touch_it(torch.bfloat16, N)
+    for N in (1, 90):
+        test_pages_that_hold_nothing_yet(N)
+    for H in (2, 16):
+        test_nan_in_a_value_reaches_its_dim_alone(H)
+    test_pages_the_table_does_not_name()
+    for N, D, ps in ((70, 64, 16), (150, 128, 32), (140, 32, 64), (300, 128, 128)):
+        test_prompt_over_a_page_without_a_name(N, D, ps)
+    for N in (1, 30, 140):
+        test_scales_far_apart_and_zero_pages(torch.float16, N)
+    test_long_flat_tail_keeps_its_weight()
+    test_sharp_rows_and_one_key()

@@ -237,3 +237,15 @@ def test_paged_attention_entry_rejects_heads_and_workspaces(lib):
         assert lib.fa_strerror(code).decode() != "unknown status"
         with pytest.raises(ValueError):
             _lib.check(code, "x")
+
+
+@pytest.mark.parametrize("rows,parts,ws,size,code", [
+    (64, 1, NULL, 0, _lib.FA_ERR_TILE), (0, 1, NULL, 0, _lib.FA_ERR_TILE),
+    (16, 0, NULL, 0, _lib.FA_ERR_UNSUPPORTED), (256, 129, FAKE, 1 << 40, _lib.FA_ERR_UNSUPPORTED),
+    (16, 2, NULL, 0, _lib.FA_ERR_WORKSPACE), (16, 2, FAKE, 2 * 2 * 16 * 68 * 4 - 1, _lib.FA_ERR_WORKSPACE),
+    (128, 3, FAKE, 2 * 3 * 128 * 68 * 4 - 1, _lib.FA_ERR_WORKSPACE), (16, 2, FAKE + 4, 1 << 40, _lib.FA_ERR_WORKSPACE),
+])
+def test_exact_cut_rejects(lib, rows, parts, ws, size, code):
+    r, c = ctypes.byref(Rows(FAKE, 512, 64, 64)), ctypes.byref(pages())
+    assert lib.fa_paged_attention_exact(r, c, FAKE, NULL, r, NULL, 1, 4, 8, 64, 0, 0.1, rows, parts, ws, size, NULL) == code
+    assert lib.fa_paged_attention_exact(r, c, FAKE, NULL, r, NULL, 1, 3, 8, 64, 0, 0.1, rows, parts, ws, size, NULL) == _lib.FA_ERR_DIMS
