@@ -42,12 +42,14 @@ __device__ __forceinline__ void decode8(const u32x2& w, float (&y)[8]) {
 // Append.  The first `items` workgroups each own one page of one sequence and K/V head, for K or for V, so
 // nobody else writes its codes and scale: it holds the page's new rows in registers, reduces their largest
 // value, and writes codes.  The others turn the queries (turn_heads); the pages, whose chain of waits is
-// longer, go first (queries first: +3 % at B=2 H=32 H_kv=8 N=8192 D=128, +5 % at N=1).  PASSES: rows of a page
-// over the rows that the workgroup's NT threads hold at once; four at most, or the registers leave too few waves
+// longer, go first (queries first: +3 % at B=2 H=32 H_kv=8 N=8192 D=128, +5 % at N=1).  PASSES: new rows of a page over
+// the rows that the workgroup's NT threads hold at once; four at most, or the registers leave too few waves
 // (128-row pages at D = 128: eight passes of 256 threads 101 us, four of 512 95; 64-row pages: four of 256 90, two
-// of 512 91), and no more threads than a page has pieces (16-row pages at D = 64, B=3 N=1000: 256 threads 9.3 us,
-// 128 7.1).  Bytes bound the large call: B=2 H=32 H_kv=8 N=8192 D=128 in pages of 128 takes 93 us, 4.05 TB/s, some 12
-// of them K's norm and table rows; one token a sequence is the chain length, page, scale, row, code (B=64: 6.8 us).
+// of 512 91), and no more threads than the new rows have pieces: where few tokens are new, the start of the waves is the
+// time (one token, B=64 D=128, pages of 128 rows: 512 threads 12.1 us, 64 5.6; with 32 K/V heads 32.6 and 6.8; 16-row
+// pages at D = 64, B=3 N=1000: 256 threads 9.3 us, 128 7.1).  Bytes bound the large call: B=2 H=32 H_kv=8 N=8192 D=128
+// in pages of 128 takes 93 us, 4.05 TB/s, some 12 of them K's norm and table rows; one token a sequence is a launch and
+// the chain length, page, scale, row, code (B=64 H=32 H_kv=8: 5.4 us).
 template <typename E, int D, bool INTER, int PASSES, int NT>
 __global__ __launch_bounds__(NT) void append_kernel(AppendArgs a, int items, int q_chunks, int touched) {
   using S = Slot<D, NT>;
@@ -76,6 +78,7 @@ __global__ __launch_bounds__(NT) void append_kernel(AppendArgs a, int items, int
   const int page = page_of(a.cache, b, col);
   if (page < 0) return;
   const int held = max(past - first, 0);           // rows the page holds already
+  const int row0 = held, n0 = first + held - past; // the page's first new row, and its token
 
   const int lane = threadIdx.x & 63;
   const int d0 = (threadIdx.x % S::TPR) * 8;
@@ -92,12 +95,11 @@ __global__ __launch_bounds__(NT) void append_kernel(AppendArgs a, int items, int
   float amax = 0.f;
   if (is_k) load_weights<INTER>(a.rot, a.rot.k_weight, d0, own, other);
   auto live = [&](int p) __attribute__((always_inline)) {
-    const int n = first + p * S::TOKENS + slot - past;
-    return p * S::TOKENS + slot < ps && n >= 0 && n < fresh;
+    return row0 + p * S::TOKENS + slot < ps && n0 + p * S::TOKENS + slot < fresh;
   };
   auto pass = [&](int p, bool all) __attribute__((always_inline)) {
     const bool mine = all || live(p);
-    const int n = mine ? first + p * S::TOKENS + slot - past : 0;
+    const int n = mine ? n0 + p * S::TOKENS + slot : 0;
     const u32x4 w = gload16(src + n * in.stride_n);
     r[p] = 1.f;
     if (is_k) {
@@ -122,8 +124,7 @@ __global__ __launch_bounds__(NT) void append_kernel(AppendArgs a, int items, int
   } else {
 #pragma unroll
     for (int p = 0; p < PASSES; ++p) {
-      const int n = first + p * S::TOKENS - past;
-      if (n + S::TOKENS > 0 && n < fresh) pass(p, false);
+      if (row0 + p * S::TOKENS < ps && n0 + p * S::TOKENS < fresh) pass(p, false);
     }
   }
   __shared__ float tops[NT / 64];
@@ -159,13 +160,23 @@ __global__ __launch_bounds__(NT) void append_kernel(AppendArgs a, int items, int
   const float mul = exp2i(-e);
 #pragma unroll
   for (int p = 0; p < PASSES; ++p)
-    if (all || live(p)) *reinterpret_cast<u32x2*>(codes + (p * S::TOKENS + slot) * D) = encode8(z[p], r[p] * mul);
+    if (all || live(p)) *reinterpret_cast<u32x2*>(codes + (row0 + p * S::TOKENS + slot) * D) = encode8(z[p], r[p] * mul);
   if (held > 0 && e > e_held) {
     const float move = exp2i(e_held - e);
-    for (int row = slot; row < held; row += S::TOKENS) {
-      float x[8];
-      decode8(*reinterpret_cast<const u32x2*>(codes + row * D), x);
-      *reinterpret_cast<u32x2*>(codes + row * D) = encode8(x, move);
+    constexpr int AHEAD = 8;   // rows in flight
+    for (int at = slot; at < held; at += AHEAD * S::TOKENS) {
+      u32x2 w[AHEAD];
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) {
+        const int row = at + i * S::TOKENS;
+        w[i] = *reinterpret_cast<const u32x2*>(codes + (row < held ? row : at) * D);
+      }
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) {
+        float x[8];
+        decode8(w[i], x);
+        if (at + i * S::TOKENS < held) *reinterpret_cast<u32x2*>(codes + (at + i * S::TOKENS) * D) = encode8(x, move);
+      }
     }
   }
   if (threadIdx.x == 0) static_cast<uint8_t*>(scales)[ph] = (uint8_t)(e + 127);
@@ -647,16 +658,18 @@ int launch_append(AppendArgs a) {
 template <typename E, int D>
 int launch_append(const AppendArgs& a) {
 #define FA_PASSES(P_, NT_) (a.rot.interleaved ? launch_append<E, D, true, P_, NT_>(a) : launch_append<E, D, false, P_, NT_>(a))
-  switch (a.cache.page_size * Slot<D>::TPR) {   // threads for a page's rows at once
-    case 64: return FA_PASSES(1, 64);
-    case 128: return FA_PASSES(1, 128);
-    case 256: return FA_PASSES(1, 256);
-    case 512: return FA_PASSES(2, 256);
-    case 1024: return FA_PASSES(4, 256);
-    case 2048: return FA_PASSES(4, 512);
-  }
+  const int at_once = std::min(a.N, a.cache.page_size) * Slot<D>::TPR;   // threads for a page's new rows at once
+  if (at_once <= 64) return FA_PASSES(1, 64);
+  if (at_once <= 128) return FA_PASSES(1, 128);
+  if (at_once <= 256) return FA_PASSES(1, 256);
+  if constexpr (D > 32)
+    if (at_once > 512) {
+      if constexpr (D > 64)
+        if (at_once > 1024) return FA_PASSES(4, 512);
+      return FA_PASSES(4, 256);
+    }
+  return FA_PASSES(2, 256);
 #undef FA_PASSES
-  return FA_ERR_UNSUPPORTED;
 }
 
 // How a call's rows and keys are cut: blocks of `rows` rows (16 and 32 to the kernel of few rows), each block's

@@ -669,3 +669,21 @@ def test_every_cut_at_every_size(rows, parts, monkeypatch):
         test_scales_far_apart_and_zero_pages(torch.float16, N)
     test_long_flat_tail_keeps_its_weight()
     test_sharp_rows_and_one_key()
+
+
+@pytest.mark.parametrize("D", [32, 64, 128])
+@pytest.mark.parametrize("ps", [16, 32, 64, 128])
+@pytest.mark.parametrize("n", [1, 2, 9, 40])
+def test_every_row_of_a_page_moves_when_its_scale_grows(D, ps, n):
+    """A page filled up to its last n rows, then n rows 2^9 as large: codes and scales as the oracle appends them."""
+    n, B, Hkv = min(n, ps - 1), 2, 3
+    k, v = (randn(i, B, Hkv, ps, D).bfloat16() for i in range(2))
+    for t in (k, v):
+        t[:, :, ps - n:] *= 512
+    bt = tables(B, 1, 2, 3)
+    cache, ref = paged_kv_cache(2, Hkv, ps, D), orc.Cache(*paged_kv_cache(2, Hkv, ps, D, device="cpu"))
+    for at, end in ((0, ps - n), (ps - n, ps)):
+        append_paged_kv(cache, k[:, :, at:end], v[:, :, at:end], bt, ints(at, at))
+        for b in range(B):
+            ref.append((k[b, :, at:end].cpu(), v[b, :, at:end].cpu()), b, bt.cpu(), at, end - at)
+    same_cache(cache, ref)
