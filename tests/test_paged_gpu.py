@@ -687,3 +687,15 @@ def test_every_row_of_a_page_moves_when_its_scale_grows(D, ps, n):
         for b in range(B):
             ref.append((k[b, :, at:end].cpu(), v[b, :, at:end].cpu()), b, bt.cpu(), at, end - at)
     same_cache(cache, ref)
+
+
+@pytest.mark.parametrize("B,Hkv,parts", [(3, 5, 5), (13, 5, 1), (8, 1, 1), (1, 7, 9), (9, 8, 2)])
+def test_parts_that_do_not_fill_the_last_round(B, Hkv, parts, monkeypatch):
+    """Row blocks by part over the eight L2s: whole rounds of eight parts, and a last one that is not."""
+    monkeypatch.setitem(globals(), "fused_paged_attention", exact_cut(16, parts))
+    ps, width, N = 16, 40, 20
+    cache = filled(B * width, Hkv, ps, 32, 80, spread=3)
+    bt = tables(B, width, B * width, 81)
+    past = ints(*((97 * b) % (width * ps - N) for b in range(B)))
+    new = ints(*(N if b % 3 else 7 * (b % 2) for b in range(B)))
+    check_attend(randn(82, B, 2 * Hkv, N, 32).half(), cache, bt, past, new)
