@@ -679,19 +679,17 @@ struct Cut {
   int rows, step, row_blocks, nsplit;
 };
 
-// Up to 16 rows, a token or a few: as many parts as give each CU a workgroup (more only divide the same bytes into
-// shorter runs and more partial rows: us at 1 / 2 / 4 workgroups to a CU, 8 sequences of 1335 to 4005 keys, 8 K/V heads,
-// D = 128: 17.4 / 20.7 / 26.4; 64 of 667 to 2000 keys 36.1 / 36.2 / 40.8; one of 16000 keys 13.8 / 15.5 / 24.9), up to
-// four where a part keeps 4096 keys, for lengths that differ (32 sequences of 5461 to 16384 keys 140.9 / 141.9 / 135.3).
-//
-// More rows: the shape and the parts of the least cost by the times below: a workgroup's start, a step of its keys where
-// each CU holds one workgroup, and on a full CU what each workgroup adds, a step and by itself; the read of the keys;
-// the join with its partial rows.  They come within 15 % (rms) of the good ones among 1500 cuts of 150 calls (2 to 3000
-// new tokens, D = 32, 64 and 128), and the cut taken is 2 % slower than the best of its call on average, 22 % at most.
+// The shape and the parts of the least cost by the times below: a workgroup's start, a step of its keys where each CU
+// holds one workgroup, and on a full CU what each workgroup adds, a step and by itself; the join with its partial rows.
+// For more than 16 rows they come within 15 % (rms) of the good ones among 1500 cuts of 150 calls (2 to 3000 new tokens,
+// D = 32, 64 and 128), and the cut taken is 2 % slower than the best of its call on average, 22 % at most.
 // Small blocks spread a short prompt over the CUs, large ones convert each key for more rows (us of blocks of 16 / 32 / 128 / 256
 // rows, D = 128, one sequence, H=32 H_kv=8, no keys before: 64 new tokens 6.4 / 7.7 / 7.4 / 9.4, 512 18.2 / 14.0 / 16.7 /
 // 20.5, 2048 119 / 75 / 53 / 57; two of 2048 235 / 151 / 87 / 77; blocks of 64 rows on four waves lay behind one of the
-// others everywhere).
+// others everywhere).  Parts fill the CUs and no more (up to 16 rows, us at 1 / 2 / 4 workgroups to a CU, 8 sequences of
+// 1335 to 4005 keys, 8 K/V heads, D = 128: 17.4 / 20.7 / 26.4; one of 16000 keys 13.8 / 15.5 / 24.9), less where the keys are
+// few (16 sequences of 160 keys, one K/V head, D = 32: filled 9.3, whole 5.5), and for lengths that differ up to four
+// workgroups to a CU where a part keeps 4096 keys (32 sequences of 5461 to 16384 keys 140.9 / 141.9 / 135.3).
 struct Shape {
   int rows, step;
   float start, one, full, each;   // us; steps at D = 128
@@ -700,34 +698,33 @@ constexpr Shape kShapes[] = {{16, kSplitStep, 6.f, 0.8f, 0.8f, 0.7f},
                              {32, kSplitStep, 7.f, 0.9f, 1.0f, 0.7f},
                              {128, kBlockKeys, 6.5f, 1.2f, 1.05f, 0.7f},
                              {256, kBlockKeys, 7.f, 1.8f, 1.9f, 3.0f}};
-constexpr int kParts[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64, 96, kMaxSplit};
+constexpr unsigned kParts[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64, 96, kMaxSplit};
 
 Cut cut_of(int B, int H, int Hkv, int N, int D, long long keys) {
   const long long rows = (long long)N * (H / Hkv), units = (long long)B * Hkv;
   const long long cus = cu_count();
   Cut c{16, kSplitStep, 1, 1};
-  if (rows <= 16) {
-    const long long fill = (cus + units - 1) / units, four = (4 * cus + units - 1) / units;
-    c.nsplit = (int)std::max<long long>(1, std::min<long long>({std::max(fill, std::min(four, keys / 4096)),
-                                                                (keys + c.step - 1) / c.step, kMaxSplit}));
-    return c;
-  }
+  const long long least = rows <= 16 ? std::min<long long>({(4 * cus + units - 1) / units, keys / 4096, kMaxSplit}) : 1;
   const float seen = 1.f - 0.5f * (float)std::min<long long>(N, keys) / (float)keys;   // of the keys, by a row on average
-  const float read = (float)(units * keys) * (float)D * (2.f / 7.0e6f);                // us at 7 TB/s, part of it from caches
   const float wide = (float)(D + 32) / 160.f, row_values = 2.5e-6f * (float)(units * rows) * (float)D;
   float best = 0.f;
   for (const Shape& s : kShapes) {
-    if (s.rows >= 2 * rows) break;
+    if (s.rows > 16 && s.rows >= 2 * rows) break;
     const long long blocks = (rows + s.rows - 1) / s.rows;
     const unsigned most = (unsigned)std::min<long long>((keys + s.step - 1) / s.step, 1u << 30);
-    for (const int n : kParts) {
+    bool first = true;
+    for (const unsigned part : kParts) {
+      const unsigned n = std::min(part, most);
       const long long wgs = units * blocks * n;
-      if (n > 1 && ((unsigned)n > most || wgs > 4 * cus)) break;
+      if (n < least && n < most) continue;
+      if (!first && wgs > 4 * cus) break;
+      first = false;
       const float load = (float)wgs / (float)cus, steps = (float)((most + n - 1) / n) * wide;
       const float on_cu = s.rows <= 32 ? load : (float)(long long)(load + 0.999f);   // (one of the large at a time)
-      const float work = std::max({steps * s.one, (steps * seen * s.full + s.each) * on_cu, read});
+      const float work = std::max(steps * s.one, (steps * seen * s.full + s.each) * on_cu);
       const float us = s.start + work + (n == 1 ? 0.f : 2.5f + row_values * (float)n);
-      if (best == 0.f || us < best) best = us, c = Cut{s.rows, s.step, (int)blocks, n};
+      if (best == 0.f || us < best) best = us, c = Cut{s.rows, s.step, (int)blocks, (int)n};
+      if (n == most) break;
     }
   }
   return c;
