@@ -10,8 +10,8 @@
 // 256 rows where there are as many: each converted tile serves twice the rows.  Products, layouts and order of a
 // step are those of the causal forward (fa_fwd.hip): S^T = K Q^T on 32x32x16 products with a lane owning one row,
 // the scores fed back as the B operand of O^T += V^T P^T, V^T read transposed from LDS, S(j + 1) under the softmax
-// of S(j).  B=2 H=32 H_kv=8, 2048 new tokens behind 6144, D=128: 418-441 us by machine,
-// 1090-1150 TFLOP/s, the matrix pipes busy 56 % of the time at 1.94 GHz.  What differs:
+// of S(j).  B=2 H=32 H_kv=8, 2048 new tokens behind 6144, D=128: 418-449 us by machine,
+// 1070-1150 TFLOP/s, the matrix pipes busy 56 % of the time at 1.94 GHz.  What differs:
 //   * a 16-key part of a tile (the whole tile with pages of 64 keys or more) lies in one page: its K scale
 //     multiplies its scores, its V scale joins their exponent, and leaves the row sums again, part by part;
 //   * pages and scales of 16 tiles (64 with pages of 64 keys or more) at a time are kept one part to a lane
